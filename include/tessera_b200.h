@@ -100,7 +100,17 @@ int tsr_synchronize(tsr_context* ctx);
  *   gemm_q4k_bf16, gemm_q6k_bf16, gemm_mxfp4_bf16, gemm_fp8_bf16: buffers A (bf16,
  *     m x k), W, [S: fp8 only], C (bf16, m x n); scalars m, n, k (k a multiple of 8).
  *     C = RoundBf16Ref (src/core/numerics/quant.cpp:231-243) of the fp32 id's sums on
- *     the same values; the reference keeps A and C in fp32 (backend.hpp:153-156). */
+ *     the same values; the reference keeps A and C in fp32 (backend.hpp:153-156);
+ *   the steps of many rows (their typed launchers below state what they compute; floats are passed as their bits):
+ *   attention_tree: buffers q, k, v, parents (int32), out; scalars m, n, heads, kv_heads, head_dim, row_base, window, kv_f16;
+ *   attention_tree_q8 / _q4 / _fp8: buffers q, k, v, k_scale, v_scale, parents, out; scalars m .. window;
+ *   qk_norm_rope: buffers q, k, q_w, k_w, pos, q_out, k_out; scalars rows, heads, kv_heads, head_dim, rope_dim, theta, sec_t,
+ *     sec_h, sec_w, eps;
+ *   qk_norm_rope_append: buffers q, k, v, q_w, k_w, pos, q_out, k_cache, v_cache; scalars as before, then cache_row, kv_f16;
+ *   qk_norm_rope_append_q8 / _q4 / _fp8: the same and k_scale, v_scale; scalars as before, then cache_row;
+ *   delta_chunk_heads: buffers S, k, v, q, o, alpha, beta, S_out; scalars heads, k_heads, dk, dv, rows, sbase, abase;
+ *   logprob_rows: buffers logits, targets (u32), logprob, entropy, top_ids (u32), top_logprobs; scalars rows, vocab, top_k,
+ *     row_base. */
 int tsr_kernel_count(void);
 const char* tsr_kernel_name(int kernel);
 int tsr_kernel_lookup(const char* name);
@@ -306,6 +316,46 @@ int tsr_attention_split(int kv_format, const float* q, const void* k, const void
  * (src/backends/rocm/rocm_kernels_basic.cpp:664-686) */
 int tsr_attention_combine(const float* pacc, const float* pmax, const float* psum, float* out, uint64_t m, uint64_t heads,
                           uint64_t head_dim, uint64_t split, void* stream);
+/* attention_tree / attention_tree_q8 / _q4 / _fp8 (this library's own): attention of the m rows of a drafted tree, to verify
+ * several continuations in one step.  The cache holds n past rows (n may be 0) and, behind them, the tree's m rows: n + m rows in
+ * kv_format.  parents[i] (device memory) is the row before i that row i continues, or -1 where it continues the past; row i
+ * sees the past, its ancestors and itself, with window != 0 the last `window` of these.  A row with any other value, or
+ * below one, is not used: it sees nothing, no row sees it, its result is 0 (trees smaller than m).  Query row i is row
+ * row_base + i of q / out (out may be q); scale, head mapping, scales of the quantised formats and limits on head_dim and heads as
+ * tsr_attention; m at most 256, else TSR_UNSUPPORTED_FEATURE.  out may not overlap anything but q in place. */
+int tsr_attention_tree(int kv_format, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                       const int32_t* parents, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
+                       uint64_t head_dim, uint64_t row_base, uint64_t window, void* stream);
+/* qk_norm_rope (this library's own): the per-head rmsnorm of rows x heads queries and rows x kv_heads keys (weights q_w, k_w of
+ * head_dim, eps >= 0) and their rotation (tsr_mrope: pos = rows x (t, h, w), sections of sec_t, sec_h, sec_w pairs) in one launch.
+ * q_out / k_out may be q / k, else nothing written may overlap anything.  head_dim at most 256, else TSR_UNSUPPORTED_FEATURE. */
+int tsr_qk_norm_rope(const float* q, const float* k, const float* q_w, const float* k_w, const uint64_t* pos, float* q_out,
+                     float* k_out, uint64_t rows, uint64_t heads, uint64_t kv_heads, uint64_t head_dim, uint64_t rope_dim,
+                     float theta, uint64_t sec_t, uint64_t sec_h, uint64_t sec_w, float eps, void* stream);
+/* qk_norm_rope_append / _q8 / _q4 / _fp8 (this library's own): the same with the rows of k (normalised, rotated) and of v written
+ * to rows cache_row.. of the key / value cache in kv_format (codes and scales as tsr_quantize_rows and
+ * tsr_quantize_fp8_pack write them; kv_heads * head_dim at most 8192 there); k itself is left as it is.  Other rows of the cache
+ * are not touched. */
+int tsr_qk_norm_rope_append(int kv_format, const float* q, const float* k, const float* v, const float* q_w, const float* k_w,
+                            const uint64_t* pos, float* q_out, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                            uint64_t rows, uint64_t cache_row, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
+                            uint64_t rope_dim, float theta, uint64_t sec_t, uint64_t sec_h, uint64_t sec_w, float eps,
+                            void* stream);
+/* delta_chunk_heads (this library's own): the rows of tsr_delta_step_heads in its chunked form, 32 rows at a time, for prompts
+ * and chains of drafted tokens.  Queries and keys are rows x k_heads x dk: value head h reads key head h % k_heads (what
+ * tsr_repeat_heads expands).  The state (heads x dk x dv) is read at s + sbase and written at s_out + sbase (which may be the same),
+ * alpha and beta are read at abase + t * heads + h; no other overlap.  dk 64 or 128 and dv % 16 == 0, else
+ * TSR_UNSUPPORTED_FEATURE.  Results agree with the row-by-row form to fp32 rounding; a value that is not finite spreads over its
+ * head's rows from the 32 it lies in on. */
+int tsr_delta_chunk_heads(const float* s, const float* k, const float* v, const float* q, float* o, const float* alpha,
+                          const float* beta, float* s_out, uint64_t heads, uint64_t k_heads, uint64_t dk, uint64_t dv,
+                          uint64_t rows, uint64_t sbase, uint64_t abase, void* stream);
+/* logprob_rows (this library's own): of rows x vocab logits (output row r: input row row_base + r) the log probability of
+ * targets[r] (-inf for an id >= vocab), the entropy (nats) and the top_k (0..32; 0: top_ids and top_logprobs may be null) largest
+ * logits' indices and log probabilities, descending, equal logits lowest index first.  A logit of -inf is a token that cannot
+ * come; a row of nothing else gives -inf and entropy 0; a row with NaN or +inf gives NaN.  Places beyond the vocabulary: id 0, -inf. */
+int tsr_logprob_rows(const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids,
+                     float* top_logprobs, uint64_t rows, uint64_t vocab, uint64_t top_k, uint64_t row_base, void* stream);
 /* silu_mul: O = silu(G) * U, backend.hpp:257-260; SiluMulRef src/core/numerics/norm.cpp:211-225 */
 int tsr_silu_mul(const float* g, const float* u, float* o, uint64_t n, void* stream);
 /* rmsnorm: Y = X / sqrt(mean(X^2) + eps) * W per row, backend.hpp:212-216; RmsNormRef

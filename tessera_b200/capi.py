@@ -108,6 +108,11 @@ SIGNATURES = {
     "tsr_attention": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _vp, _vp] + [_u64] * 9 + [_vp]),
     "tsr_attention_split": (C.c_int, [C.c_int] + [_vp] * 8 + [_u64] * 9 + [_vp]),
     "tsr_attention_combine": (C.c_int, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _vp]),
+    "tsr_attention_tree": (C.c_int, [C.c_int] + [_vp] * 7 + [_u64] * 7 + [_vp]),
+    "tsr_qk_norm_rope": (C.c_int, [_vp] * 7 + [_u64] * 5 + [C.c_float] + [_u64] * 3 + [C.c_float, _vp]),
+    "tsr_qk_norm_rope_append": (C.c_int, [C.c_int] + [_vp] * 11 + [_u64] * 6 + [C.c_float] + [_u64] * 3 + [C.c_float, _vp]),
+    "tsr_delta_chunk_heads": (C.c_int, [_vp] * 8 + [_u64] * 7 + [_vp]),
+    "tsr_logprob_rows": (C.c_int, [_vp] * 6 + [_u64] * 4 + [_vp]),
     "tsr_mrope": (C.c_int, [_vp, _vp, _u64, _u64, _u64, _u64, C.c_float, _u64, _u64, _u64, _vp]),
     "tsr_cast_f32_f16": (C.c_int, [_vp, _vp, _u64, _vp]),
     "tsr_delta_step_heads": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _vp]),

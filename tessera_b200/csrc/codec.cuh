@@ -68,6 +68,17 @@ __device__ __forceinline__ uint32_t float_to_e4m3_ref(float v) {
   return sign | (static_cast<uint32_t>(field) << 3) | static_cast<uint32_t>(man);
 }
 
+// The code float_to_e4m3_ref gives a value in [-448, 448] (or a NaN), from the hardware's conversion: both round to
+// nearest even, but the reference clamps a subnormal's mantissa at 7 where rounding would carry into the smallest normal
+// value, and keeps a NaN's sign.
+__device__ __forceinline__ uint32_t e4m3_code(float q) {
+  const uint32_t bits = __float_as_uint(q), sign = (bits >> 31) << 7;
+  const float mag = fabsf(q);
+  uint32_t code = __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+  if (mag >= 7.5f / 512.0f && mag < 8.0f / 512.0f) code = sign | 7u;
+  return q == q ? code : (sign | 0x7Fu);
+}
+
 // Scale/min pair j of a Q4_K block from the 12 packed bytes held as three
 // little-endian words (src/core/numerics/quant.cpp:58-70).
 __device__ __forceinline__ void q4k_scale_min(const uint32_t s[3], int j, uint32_t& sc,

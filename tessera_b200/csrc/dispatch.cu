@@ -711,6 +711,95 @@ int k_attention_combine(const Args& a) {
   return tsr_attention_combine(f(0), f(1), f(2), f(3), m, heads, d, split, a.stream);
 }
 
+// ---- the steps of many rows (ids of this library; tessera_b200.h states their buffers and scalars) ----
+
+// attention_tree (KIND -1: fp32 or fp16 cache), attention_tree_q8 / _q4 / _fp8
+template <int KIND>
+int k_attention_tree(const Args& a) {
+  constexpr bool kQuant = KIND >= 0;
+  if (!shape(a, kQuant ? 7 : 5, kQuant ? 7 : 8)) return kInvalidArgument;
+  const uint64_t m = a.sc[0], n = a.sc[1], heads = a.sc[2], kvh = a.sc[3], d = a.sc[4], rb = a.sc[5], win = a.sc[6];
+  if (n > kMaxDim || !attention_dims_ok(m, n + 1, heads, kvh, d, rb, win)) return kInvalidArgument;
+  if (!attention_served(heads, kvh, d) || m > 256) return kUnsupportedFeature;
+  const int fmt = kQuant ? kQuantKv[kQuant ? KIND : 0] : a.sc[7] != 0 ? TSR_KV_F16 : TSR_KV_F32;
+  const uint64_t cache = cache_bytes(fmt, (n + m) * kvh * d), rows = (rb + m) * heads * d * 4;
+  const int par = kQuant ? 5 : 3;
+  if (!holds(a, 0, rows) || !holds(a, 1, cache) || !holds(a, 2, cache) || !holds(a, par, m * 4) || !holds(a, par + 1, rows) ||
+      (kQuant && (!holds(a, 3, (n + m) * 4) || !holds(a, 4, (n + m) * 4))))
+    return kInvalidArgument;
+  return attention_tree(fmt, static_cast<const float*>(a.buf[0]), a.buf[1], a.buf[2], kQuant ? static_cast<const float*>(a.buf[3]) : nullptr,
+                            kQuant ? static_cast<const float*>(a.buf[4]) : nullptr, static_cast<const int32_t*>(a.buf[par]),
+                            static_cast<float*>(const_cast<void*>(a.buf[par + 1])), m, n, heads, kvh, d, rb, win, a.dry, a.stream);
+}
+
+// qk_norm_rope and qk_norm_rope_append* share their first scalars: rows, heads, kv_heads, head_dim, rope_dim, theta, sections, eps
+bool norm_rope_dims_ok(const Args& a) {
+  const uint64_t rows = a.sc[0], heads = a.sc[1], kvh = a.sc[2], d = a.sc[3], rdim = a.sc[4];
+  const float theta = float_of_bits(a.sc[5]), eps = float_of_bits(a.sc[9]);
+  return dims_ok(rows, heads, kvh) && heads <= 65535 && kvh <= 65535 && d > 0 && d <= 65535 && d % 2 == 0 && rdim != 0 && rdim <= d &&
+         rdim % 2 == 0 && a.sc[6] <= rdim && a.sc[7] <= rdim && a.sc[8] <= rdim && a.sc[6] + a.sc[7] + a.sc[8] <= rdim / 2 &&
+         theta > 0.0f && theta <= 3.4028235e38f && eps >= 0.0f;
+}
+
+int k_qk_norm_rope(const Args& a) {
+  if (!shape(a, 7, 10) || !norm_rope_dims_ok(a)) return kInvalidArgument;
+  const uint64_t rows = a.sc[0], heads = a.sc[1], kvh = a.sc[2], d = a.sc[3];
+  if (d > 256) return kUnsupportedFeature;
+  if (!holds(a, 0, rows * heads * d * 4) || !holds(a, 1, rows * kvh * d * 4) || !holds(a, 2, d * 4) || !holds(a, 3, d * 4) ||
+      !holds(a, 4, rows * 24) || !holds(a, 5, rows * heads * d * 4) || !holds(a, 6, rows * kvh * d * 4))
+    return kInvalidArgument;
+  auto f = [&](int i) { return static_cast<float*>(const_cast<void*>(a.buf[i])); };
+  return qk_norm_rope(f(0), f(1), f(2), f(3), static_cast<const uint64_t*>(a.buf[4]), f(5), f(6), rows, heads, kvh, d, a.sc[4],
+                          float_of_bits(a.sc[5]), a.sc[6], a.sc[7], a.sc[8], float_of_bits(a.sc[9]), a.dry, a.stream);
+}
+
+template <int KIND>
+int k_qk_norm_rope_append(const Args& a) {
+  constexpr bool kQuant = KIND >= 0;
+  if (!shape(a, kQuant ? 11 : 9, kQuant ? 11 : 12) || !norm_rope_dims_ok(a)) return kInvalidArgument;
+  const uint64_t rows = a.sc[0], heads = a.sc[1], kvh = a.sc[2], d = a.sc[3], at = a.sc[10], cols = kvh * d;
+  const int fmt = kQuant ? kQuantKv[kQuant ? KIND : 0] : a.sc[11] != 0 ? TSR_KV_F16 : TSR_KV_F32;
+  if (at > kMaxDim || (kQuant && cols % (fmt == TSR_KV_INT4 ? 8 : 4) != 0)) return kInvalidArgument;
+  if (d > 256 || (kQuant && cols > 8192)) return kUnsupportedFeature;
+  const uint64_t cache = cache_bytes(fmt, (at + rows) * cols);
+  if (!holds(a, 0, rows * heads * d * 4) || !holds(a, 1, rows * cols * 4) || !holds(a, 2, rows * cols * 4) || !holds(a, 3, d * 4) ||
+      !holds(a, 4, d * 4) || !holds(a, 5, rows * 24) || !holds(a, 6, rows * heads * d * 4) || !holds(a, 7, cache) || !holds(a, 8, cache) ||
+      (kQuant && (!holds(a, 9, (at + rows) * 4) || !holds(a, 10, (at + rows) * 4))))
+    return kInvalidArgument;
+  auto f = [&](int i) { return static_cast<float*>(const_cast<void*>(a.buf[i])); };
+  return qk_norm_rope_append(fmt, f(0), f(1), f(2), f(3), f(4), static_cast<const uint64_t*>(a.buf[5]), f(6), const_cast<void*>(a.buf[7]),
+                                 const_cast<void*>(a.buf[8]), kQuant ? f(9) : nullptr, kQuant ? f(10) : nullptr, rows, at, heads, kvh, d, a.sc[4],
+                                 float_of_bits(a.sc[5]), a.sc[6], a.sc[7], a.sc[8], float_of_bits(a.sc[9]), a.dry, a.stream);
+}
+
+int k_delta_chunk_heads(const Args& a) {
+  if (!shape(a, 8, 7)) return kInvalidArgument;
+  const uint64_t heads = a.sc[0], kh = a.sc[1], dk = a.sc[2], dv = a.sc[3], rows = a.sc[4], sbase = a.sc[5], abase = a.sc[6];
+  if (!dims_ok(heads, dk, dv) || !dims_ok(kh, rows, 1) || heads > 65535 || dk > 65535 || dv > 65535 || heads % kh != 0 || sbase > kMaxDim * 1024 ||
+      abase > kMaxDim * 1024)
+    return kInvalidArgument;
+  if ((dk != 64 && dk != 128) || dv % 16 != 0) return kUnsupportedFeature;
+  const uint64_t state = (sbase + heads * dk * dv) * 4;
+  if (!holds(a, 0, state) || !holds(a, 1, rows * kh * dk * 4) || !holds(a, 2, rows * heads * dv * 4) || !holds(a, 3, rows * kh * dk * 4) ||
+      !holds(a, 4, rows * heads * dv * 4) || !holds(a, 5, (abase + rows * heads) * 4) || !holds(a, 6, (abase + rows * heads) * 4) ||
+      !holds(a, 7, state))
+    return kInvalidArgument;
+  auto f = [&](int i) { return static_cast<float*>(const_cast<void*>(a.buf[i])); };
+  return delta_chunk_heads(f(0), f(1), f(2), f(3), f(4), f(5), f(6), f(7), heads, kh, dk, dv, rows, sbase, abase, a.dry, a.stream);
+}
+
+int k_logprob_rows(const Args& a) {
+  if (!shape(a, 6, 4)) return kInvalidArgument;
+  const uint64_t rows = a.sc[0], vocab = a.sc[1], top_k = a.sc[2], base = a.sc[3];
+  if (!dims_ok(rows, vocab, 1) || rows > 65535 || vocab > kMaxDim - 8192 || top_k > 32 || base > kMaxDim) return kInvalidArgument;
+  if (!holds(a, 0, (base + rows) * vocab * 4) || !holds(a, 1, rows * 4) || !holds(a, 2, rows * 4) || !holds(a, 3, rows * 4) ||
+      !holds(a, 4, rows * top_k * 4) || !holds(a, 5, rows * top_k * 4))
+    return kInvalidArgument;
+  auto f = [&](int i) { return static_cast<float*>(const_cast<void*>(a.buf[i])); };
+  return logprob_rows(f(0), static_cast<const uint32_t*>(a.buf[1]), f(2), f(3), static_cast<uint32_t*>(const_cast<void*>(a.buf[4])), f(5),
+                          rows, vocab, top_k, base, a.dry, a.stream);
+}
+
 // fill: buffer int32; scalars value, count (backend.hpp:151-152).
 int k_fill(const Args& a) {
   if (!shape(a, 1, 2)) return kInvalidArgument;
@@ -957,6 +1046,17 @@ const Entry kTable[] = {
     {"attention_q4_split", k_attention_quant_split<1>},
     {"attention_fp8_split", k_attention_quant_split<2>},
     {"attention_combine", k_attention_combine},
+    {"attention_tree", k_attention_tree<-1>},
+    {"attention_tree_q8", k_attention_tree<0>},
+    {"attention_tree_q4", k_attention_tree<1>},
+    {"attention_tree_fp8", k_attention_tree<2>},
+    {"qk_norm_rope", k_qk_norm_rope},
+    {"qk_norm_rope_append", k_qk_norm_rope_append<-1>},
+    {"qk_norm_rope_append_q8", k_qk_norm_rope_append<0>},
+    {"qk_norm_rope_append_q4", k_qk_norm_rope_append<1>},
+    {"qk_norm_rope_append_fp8", k_qk_norm_rope_append<2>},
+    {"delta_chunk_heads", k_delta_chunk_heads},
+    {"logprob_rows", k_logprob_rows},
     {"copy_d2d", k_copy_d2d},
     {"mrope", k_mrope},
     {"rope", k_rope},

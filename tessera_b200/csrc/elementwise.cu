@@ -48,17 +48,6 @@ quantize_fp8_kernel(float* __restrict__ data, const float* __restrict__ in,
   }
 }
 
-// The code float_to_e4m3_ref gives a value in [-448, 448] (or a NaN), from the hardware's conversion: both round to
-// nearest even, but the reference clamps a subnormal's mantissa at 7 where rounding would carry into the smallest normal
-// value, and keeps a NaN's sign.
-__device__ __forceinline__ uint32_t e4m3_code(float q) {
-  const uint32_t bits = __float_as_uint(q), sign = (bits >> 31) << 7;
-  const float mag = fabsf(q);
-  uint32_t code = __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-  if (mag >= 7.5f / 512.0f && mag < 8.0f / 512.0f) code = sign | 7u;
-  return q == q ? code : (sign | 0x7Fu);
-}
-
 // The codes of a batch (quantize_fp8_pack) with several CTAs per row: each finds the row's maximum by itself (the row is
 // a few tens of KB, served from L2 after the first) and codes its share, four columns a thread.  One CTA a row left 16
 // verify rows on 16 SMs, with frexp and a 64-bit rounding an element: 16 rows of 5120 / 17408 took 7.3 / 17.6 us, here

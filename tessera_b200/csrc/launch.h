@@ -288,6 +288,22 @@ int launch_moe_scale_add_add(const float* a, const float* b, const float* f, flo
 int attention_gated(int kv_format, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                     float* out, const float* gate, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
                     uint64_t q_base, uint64_t row_base, uint64_t window, uint64_t causal, cudaStream_t st);
+// The steps of many rows: the typed launchers of the same names (tessera_b200.h); dry: the checks of their arguments alone.
+int attention_tree(int kv_format, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                   const int32_t* parents, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
+                   uint64_t row_base, uint64_t window, bool dry, cudaStream_t st);
+int qk_norm_rope(const float* q, const float* k, const float* q_w, const float* k_w, const uint64_t* pos, float* q_out, float* k_out, uint64_t rows,
+                 uint64_t heads, uint64_t kv_heads, uint64_t head_dim, uint64_t rope_dim, float theta, uint64_t sec_t, uint64_t sec_h,
+                 uint64_t sec_w, float eps, bool dry, cudaStream_t st);
+int qk_norm_rope_append(int kv_format, const float* q, const float* k, const float* v, const float* q_w, const float* k_w, const uint64_t* pos,
+                        float* q_out, void* k_cache, void* v_cache, float* k_scale, float* v_scale, uint64_t rows, uint64_t cache_row,
+                        uint64_t heads, uint64_t kv_heads, uint64_t head_dim, uint64_t rope_dim, float theta, uint64_t sec_t, uint64_t sec_h,
+                        uint64_t sec_w, float eps, bool dry, cudaStream_t st);
+int delta_chunk_heads(const float* s, const float* k, const float* v, const float* q, float* o, const float* alpha, const float* beta, float* s_out,
+                      uint64_t heads, uint64_t k_heads, uint64_t dk, uint64_t dv, uint64_t rows, uint64_t sbase, uint64_t abase, bool dry,
+                      cudaStream_t st);
+int logprob_rows(const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids, float* top_logprobs, uint64_t rows,
+                 uint64_t vocab, uint64_t top_k, uint64_t row_base, bool dry, cudaStream_t st);
 // Point the kernels of each file at the host-visible error word (see pipeline.cuh); once per device.
 int staged_set_error_word(unsigned int* word);
 int staged_q6k_set_error_word(unsigned int* word);

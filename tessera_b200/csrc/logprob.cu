@@ -1,0 +1,347 @@
+// Log probabilities of given tokens, the entropy of every row and its likeliest tokens, in one pass over the logits (id
+// "logprob_rows"): what a server answers beside a token, and what a verified tree's drafts or a scored prompt are judged by.
+//   lse = m + log S, m = max x, S = sum e^(x - m);   logprob = x_t - lse;   entropy = log S - T / S, T = sum e^(x - m) (x - m)
+// The reference has top_k_rows for the likeliest tokens alone (src/backends/rocm/rocm_kernels.hpp:558-566), whose kernel walks
+// a row once for every one of them.
+//
+// Bound: the logits' bytes (256 rows of 151936: 156 MB, 24 us at the measured copy rate).  A cluster of CTAs takes a row.  A
+// CTA walks over its share in tiles of 8192 logits held in registers, the next tile's loads under way, with a running maximum
+// and two running sums a thread.  The likeliest tokens come out of the same registers: a logit below the threshold -- the
+// top_k-th largest so far -- costs one comparison; the few above it go to a list in shared memory, which is cut back to its
+// top_k largest by counting, for each entry, the entries above it.  An entry is its logit's bits in an order-preserving form
+// over its inverted index, so that no two are equal and the lowest index wins among equal logits.  The first threshold is a
+// bound from the threads' maxima (enough threads are above it), and a tile that floods the list all the same (ascending or
+// equal logits) finds its own threshold by bisection over the entries.  The CTAs meet through distributed shared memory.
+#include <cuda_runtime.h>
+
+#include "codec.cuh"
+#include "launch.h"
+#include "tessera_b200.h"
+
+namespace tsr {
+namespace {
+
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32;
+constexpr int kLpPer = 16, kLpTile = kLpThreads * kLpPer;
+constexpr int kLpList = 1024;  // entries of the list: two a thread when it is cut back
+constexpr int kLpTop = 32;     // top_k at most, as top_k_rows
+constexpr int kLpCluster = 8;  // CTAs of a row at most (the portable cluster size)
+constexpr int kLpCut = 192;    // entries from which the list is cut back before the next tile
+
+using Entry64 = unsigned long long;
+
+// An order-preserving form of a logit (NaN lowest, -0 as 0), and its inverse.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return x != x ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return k == 0 ? __uint_as_float(0x7FC00000u) : __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
+}
+__device__ __forceinline__ Entry64 entry_of(float x, uint32_t index) { return static_cast<Entry64>(order_of(x)) << 32 | (0xFFFFFFFFu - index); }
+
+struct Sums {  // of e^(x - top) and of e^(x - top) (x - top); top is -inf before the first finite logit
+  float top, s, t;
+};
+__device__ __forceinline__ float shift_of(float top) { return top == -INFINITY ? 0.0f : top; }
+__device__ __forceinline__ Sums moved(const Sums& a, float top) {  // top >= a.top
+  const float by = shift_of(a.top) - shift_of(top);
+  if (a.s == 0.0f) return Sums{top, a.s, a.t};  // (nothing so far; its top may be -inf)
+  const float f = exp2f(by * 1.4426950408889634f);
+  return Sums{top, a.s * f, f == 0.0f ? 0.0f : f * fmaf(a.s, by, a.t)};  // (by may be -inf: logits of the type's lowest value)
+}
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
+  const float top = fmaxf(a.top, b.top);
+  const Sums x = moved(a, top), y = moved(b, top);
+  return Sums{top, x.s + y.s, x.t + y.t};
+}
+
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ uint32_t peer_at(uint32_t local, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+struct LogprobShared {
+  Entry64 list[kLpList], cut[kLpTop];
+  Sums sums[kLpWarps], all;
+  uint32_t bound[kLpWarps];
+  int count;
+  int had;  // entries before the tile at hand (fewer than kLpCut)
+};
+
+// The list's top_k largest to its front, in order; returns the entry that a new one has to exceed (0: none).
+__device__ __forceinline__ Entry64 cut_back(LogprobShared& sh, int n, int top_k) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int r = 0; r < kLpList / kLpThreads; ++r) {
+    const int i = tid + r * kLpThreads;
+    if (i >= n) break;
+    const Entry64 mine = sh.list[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += sh.list[j] > mine ? 1 : 0;
+    if (above < top_k) sh.cut[above] = mine;
+  }
+  __syncthreads();
+  const int left = min(n, top_k);
+  if (tid < left) sh.list[tid] = sh.cut[tid];
+  if (tid == 0) sh.count = left;
+  const Entry64 least = n >= top_k ? sh.cut[top_k - 1] : 0;
+  __syncthreads();
+  return least;
+}
+
+// grid: (cluster size, rows) in clusters along x
+template <int VEC>
+__global__ void __launch_bounds__(kLpThreads, 2)
+logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict__ targets, float* __restrict__ logprob,
+                    float* __restrict__ entropy, uint32_t* __restrict__ top_ids, float* __restrict__ top_logprobs, uint32_t vocab,
+                    int top_k, size_t row_base) {
+  __shared__ LogprobShared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = blockIdx.x, ranks = gridDim.x;
+  const size_t row = blockIdx.y;
+  const float* x = logits + (row_base + row) * vocab;
+  const uint32_t share = ((vocab + ranks - 1) / ranks + 3) / 4 * 4;
+  const uint32_t begin = min(vocab, rank * share), end = min(vocab, begin + share);
+  constexpr int kRuns = kLpPer / VEC;
+  float next[kLpPer];
+  auto index_of = [&](uint32_t tile, int i) { return tile + (i / VEC) * (kLpThreads * VEC) + tid * VEC + i % VEC; };
+  auto load = [&](uint32_t tile) {
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      const uint32_t at = index_of(tile, r * VEC);
+      if constexpr (VEC == 4) {
+        float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (at < end) y = __ldcs(reinterpret_cast<const float4*>(x + at));
+        next[r * 4] = y.x, next[r * 4 + 1] = y.y, next[r * 4 + 2] = y.z, next[r * 4 + 3] = y.w;
+      } else {
+        next[r] = at < end ? __ldcs(x + at) : -INFINITY;
+      }
+    }
+  };
+  if (tid == 0) sh.count = sh.had = 0;
+  load(begin);
+  Sums mine{-INFINITY, 0.0f, 0.0f};
+  Entry64 least = 0;             // a new entry has to exceed it
+  float threshold = -INFINITY;  // its logit
+  __syncthreads();
+  for (uint32_t tile = begin; tile < end; tile += kLpTile) {
+    float v[kLpPer];
+#pragma unroll
+    for (int i = 0; i < kLpPer; ++i) v[i] = next[i];
+    if (tile + kLpTile < end) load(tile + kLpTile);
+    const uint32_t held = min(end - tile, static_cast<uint32_t>(kLpTile));
+    float most = v[0];
+#pragma unroll
+    for (int i = 1; i < kLpPer; ++i) most = fmaxf(most, v[i]);
+    if (most > mine.top) mine = moved(mine, most);
+    const float shift = shift_of(mine.top);
+#pragma unroll
+    for (int i = 0; i < kLpPer; ++i) {
+      const float y = v[i] - shift, e = exp2f(y * 1.4426950408889634f);
+      mine.s += e;
+      mine.t = fmaf(e, fmaxf(y, -1e30f), mine.t);  // a masked logit is 0 * -1e30
+    }
+    if (top_k == 0) continue;
+    if (tile == begin) {
+      // The full[] warps whose every lane holds logits each give the per_warp-th largest of their lanes' maxima: at least
+      // top_k logits are not below the least of these.
+      const uint32_t full = held / (32 * VEC) < kLpWarps ? held / (32 * VEC) : kLpWarps;
+      uint32_t bound = 0;
+      if (full != 0) {
+        const int per_warp = (top_k + static_cast<int>(full) - 1) / static_cast<int>(full);
+        uint32_t key = order_of(most);
+        for (int r = 0; r < per_warp; ++r) {
+          bound = __reduce_max_sync(0xFFFFFFFFu, key);
+          const uint32_t who = __ballot_sync(0xFFFFFFFFu, key == bound);
+          if (lane == __ffs(who) - 1) key = 0;
+        }
+        if (lane == 0) sh.bound[warp] = bound;
+        __syncthreads();
+        bound = sh.bound[0];
+        for (uint32_t w = 1; w < full; ++w) bound = min(bound, sh.bound[w]);
+      }
+      least = bound == 0 ? 0 : static_cast<Entry64>(bound) << 32;
+      threshold = bound == 0 ? -INFINITY : value_of(bound);
+    }
+    uint32_t above = 0;
+#pragma unroll
+    for (int i = 0; i < kLpPer; ++i)
+      if (!(v[i] < threshold)) above |= 1u << i;
+    if (above != 0) {
+#pragma unroll
+      for (int i = 0; i < kLpPer; ++i) {
+        const uint32_t at = index_of(tile, i);
+        if ((above >> i & 1u) && (at >= end || entry_of(v[i], at) <= least)) above &= ~(1u << i);
+      }
+      if (above != 0) {
+        int slot = atomicAdd(&sh.count, __popc(above));
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i)
+          if (above >> i & 1u) {
+            if (slot < kLpList) sh.list[slot] = entry_of(v[i], index_of(tile, i));
+            ++slot;
+          }
+      }
+    }
+    __syncthreads();
+    int n = sh.count;
+    if (n > kLpList) {
+      // The list overflowed: its first entries are the ones it had, at most kLpCut; what this tile added is found again.
+      // Bisection for the top_k-th largest entry of both.
+      const int had = sh.had;
+      Entry64 lo = 0;
+      for (int bit = 63; bit >= 0; --bit) {
+        const Entry64 trial = lo | (1ull << bit);
+        int mine_above = tid < had && sh.list[tid] >= trial ? 1 : 0;
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i)
+          if ((above >> i & 1u) && entry_of(v[i], index_of(tile, i)) >= trial) ++mine_above;
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        mine_above = __reduce_add_sync(0xFFFFFFFFu, mine_above);
+        if (lane == 0 && mine_above != 0) atomicAdd(&sh.count, mine_above);
+        __syncthreads();
+        if (sh.count >= top_k) lo = trial;
+        __syncthreads();
+      }
+      Entry64 kept = 0;
+      if (tid < had) kept = sh.list[tid];
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      if (tid < had && kept >= lo) sh.list[atomicAdd(&sh.count, 1)] = kept;
+#pragma unroll
+      for (int i = 0; i < kLpPer; ++i) {
+        const Entry64 e = entry_of(v[i], index_of(tile, i));
+        if ((above >> i & 1u) && e >= lo) sh.list[atomicAdd(&sh.count, 1)] = e;
+      }
+      __syncthreads();
+      n = sh.count;
+    }
+    if (tile == begin || n >= kLpCut || tile + kLpTile >= end) {
+      const Entry64 cut = cut_back(sh, n, top_k);
+      if (cut != 0) least = cut, threshold = value_of(static_cast<uint32_t>(cut >> 32));
+      n = min(n, top_k);
+    }
+    if (tid == 0) sh.had = n;
+    __syncthreads();
+  }
+
+  // the threads' sums, then the CTAs'
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Sums other{__shfl_xor_sync(0xFFFFFFFFu, mine.top, o), __shfl_xor_sync(0xFFFFFFFFu, mine.s, o), __shfl_xor_sync(0xFFFFFFFFu, mine.t, o)};
+    mine = (lane & o) == 0 ? joined(mine, other) : joined(other, mine);
+  }
+  if (lane == 0) sh.sums[warp] = mine;
+  __syncthreads();
+  if (tid == 0) {
+    Sums all = sh.sums[0];
+    for (int w = 1; w < kLpWarps; ++w) all = joined(all, sh.sums[w]);
+    sh.all = all;
+  }
+  if (ranks > 1) {
+    cluster_meet();
+    if (rank == 0) {
+      if (tid == 0) {
+        Sums all = sh.all;
+        for (uint32_t r = 1; r < ranks; ++r) {
+          const uint32_t at = peer_at(shared_at(&sh.all), r);
+          Sums other;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.top) : "r"(at) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.s) : "r"(at + 4) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.t) : "r"(at + 8) : "memory");
+          all = joined(all, other);
+        }
+        sh.all = all;
+      }
+      if (tid >= top_k && tid < static_cast<int>(ranks) * top_k) {
+        const uint32_t r = tid / top_k, i = tid % top_k;
+        uint32_t n;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(peer_at(shared_at(&sh.count), r)) : "memory");
+        Entry64 e = 0;
+        if (i < n) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(e) : "r"(peer_at(shared_at(&sh.list[i]), r)) : "memory");
+        sh.list[tid] = e != 0 ? e : tid;  // below every entry, and no two alike
+      }
+      if (tid < top_k && tid >= sh.count) sh.list[tid] = tid;
+      __syncthreads();
+      if (top_k != 0) cut_back(sh, static_cast<int>(ranks) * top_k, top_k);
+    }
+    cluster_meet();  // the others' shared memory is read until here
+    if (rank != 0) return;
+  } else {
+    if (tid < top_k && tid >= sh.count) sh.list[tid] = tid;
+    __syncthreads();
+  }
+  const Sums all = sh.all;
+  const bool nothing = all.s == 0.0f;  // every logit is -inf
+  const float log_s = logf(all.s), top = shift_of(all.top);
+  if (tid == 0) {
+    const uint32_t t = targets[row];
+    logprob[row] = nothing || t >= vocab ? (all.s == all.s ? -INFINITY : all.s) : (x[t] - top) - log_s;
+    entropy[row] = nothing ? 0.0f : log_s - all.t / all.s;
+  }
+  if (tid < top_k) {
+    const Entry64 e = sh.list[tid];
+    const bool some = e >= kLpThreads;  // (a place without an entry holds its number: the row has fewer logits than top_k)
+    top_ids[row * top_k + tid] = some ? 0xFFFFFFFFu - static_cast<uint32_t>(e) : 0u;
+    top_logprobs[row * top_k + tid] = all.s != all.s ? all.s : !some || nothing ? -INFINITY : (value_of(static_cast<uint32_t>(e >> 32)) - top) - log_s;
+  }
+}
+
+// CTAs of a row: as many as the machine has room for at two a SM, while each has half a tile.
+unsigned logprob_ctas(uint64_t rows, uint64_t vocab) {
+  unsigned ctas = 1;
+  while (ctas < kLpCluster && rows * ctas * 2 <= 296 && vocab / (ctas * 2) >= kLpTile / 2) ctas *= 2;
+  return ctas;
+}
+
+}  // namespace
+
+int logprob_rows(const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids,
+                                float* top_logprobs, uint64_t rows, uint64_t vocab, uint64_t top_k, uint64_t row_base, bool dry, cudaStream_t st) {
+  if (!logits || !targets || !logprob || !entropy || rows == 0 || rows > 65535 || vocab == 0 || vocab > 0x7FFFFFFFull - kLpTile || top_k > kLpTop ||
+      row_base > 0x7FFFFFFFull || (top_k != 0 && (!top_ids || !top_logprobs)))
+    return kInvalidArgument;
+  struct {
+    const void* at;
+    uint64_t bytes;
+  } const in[2] = {{logits + row_base * vocab, rows * vocab * 4}, {targets, rows * 4}},
+          out[4] = {{logprob, rows * 4}, {entropy, rows * 4}, {top_ids, rows * top_k * 4}, {top_logprobs, rows * top_k * 4}};
+  auto meet = [](const auto& a, const auto& b) {
+    const auto *x = static_cast<const unsigned char*>(a.at), *y = static_cast<const unsigned char*>(b.at);
+    return x < y + b.bytes && y < x + a.bytes;
+  };
+  for (int i = 0; i < 4; ++i) {  // a row's results are written while others are read
+    for (const auto& r : in)
+      if (meet(out[i], r)) return kInvalidArgument;
+    for (int j = 0; j < i; ++j)
+      if (meet(out[i], out[j])) return kInvalidArgument;
+  }
+  if (dry) return kOk;
+  const unsigned ctas = logprob_ctas(rows, vocab);
+  const dim3 grid(ctas, static_cast<unsigned>(rows));
+  const bool wide = vocab % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15u) == 0;
+  const cudaError_t e = wide ? launch_kernel_cluster(logprob_rows_kernel<4>, grid, dim3(kLpThreads), 0, st, false, ctas, logits, targets, logprob,
+                                                    entropy, top_ids, top_logprobs, static_cast<uint32_t>(vocab), static_cast<int>(top_k), row_base)
+                            : launch_kernel_cluster(logprob_rows_kernel<1>, grid, dim3(kLpThreads), 0, st, false, ctas, logits, targets, logprob,
+                                                    entropy, top_ids, top_logprobs, static_cast<uint32_t>(vocab), static_cast<int>(top_k), row_base);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return kDeviceError;
+  }
+  return check_launch();
+}
+
+}  // namespace tsr
+
+extern "C" int tsr_logprob_rows(const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids,
+                                float* top_logprobs, uint64_t rows, uint64_t vocab, uint64_t top_k, uint64_t row_base, void* stream) {
+  return tsr::logprob_rows(logits, targets, logprob, entropy, top_ids, top_logprobs, rows, vocab, top_k, row_base, false,
+                           static_cast<cudaStream_t>(stream));
+}
