@@ -9,9 +9,13 @@
 #include "attention.cuh"
 #include "codec.cuh"
 #include "launch.h"
+#include "pipeline.cuh"
 #include "tessera_b200.h"
 
 namespace tsr {
+
+__device__ unsigned int g_tree_timeouts = 0;
+
 namespace {
 
 constexpr int kTreeRows = 256;  // of a tree at most
@@ -117,15 +121,815 @@ __global__ void __launch_bounds__(kTreeWarps * 32) attention_tree_rows_kernel(co
   }
 }
 
+// ---- the tensor kernel ----
+// A CTA takes 128 (tree row, head) pairs of one kv head and walks over its share of the keys in tiles of 64, on tcgen05 binary16
+// MMAs with fp32 accumulators.  Cache elements are exact in binary16 (fp32 ones are two terms of a row scaled by a power of
+// two), a query element or a softmax weight is two terms, as in attention_tile.cu.  Everything the MMAs take from the left
+// lies in tensor memory: the queries' two terms for the whole call (an operand A in shared memory would be read again for every 64
+// columns, 48 cycles where the product takes 16), a tile's weights.  Columns of tensor memory: queries 256, scores 64, weights
+// 64, and 128 for the outputs of a tile, which are read after every tile -- half of head_dim at a time -- and added to
+// fp32 registers, so that what an accumulator cuts off does not add up over the keys.
+//   warps 0-7   a thread a row (tensor memory lane), warps 0-3 keys 0-31 of a tile and outputs 0-63 of a half, 4-7 the rest
+//   warps 8-10  keys and values: global memory -> binary16 in the operands' layout
+//   warp 11     one thread issues the MMAs: outputs' first half, the next scores, outputs' second half
+constexpr int kSoftThreads = 256, kLoadThreads = 96, kTcThreads = kSoftThreads + kLoadThreads + 32;
+constexpr int kTcRows = 128, kTcKeys = 64;
+constexpr uint32_t kColQ = 0, kColS = 256, kColP = 320, kColO = 384;  // of tensor memory
+constexpr int kScaleBufs = 4;
+
+struct TcParams {
+  TreeParams t;
+  float *pacc, *pmax, *psum;  // partials of chunks as in AttnParams; null: one chunk, the result itself
+  int group, row_tiles, splits, tiles_per_split, first_key;
+};
+
+template <int KV, int D>
+struct TcShape {
+  static constexpr int kTerms = KV == kKvF32 ? 2 : 1;
+  static constexpr int kKBufs = KV == kKvF32 ? 1 : 2, kVBufs = 2;  // of a tile's keys and of its values
+  static constexpr int kTermBytes = kTcKeys * D * 2, kTileBytes = kTerms * kTermBytes;
+  static constexpr int kRowBytes = D * kv_bits<KV>() / 8;
+  static constexpr bool kRaw = KV != kKvF32 && KV != kKvF16;          // raw bytes pass through shared memory
+  static constexpr int kRawBytes = kRaw ? kTcKeys * kRowBytes : 0;
+  static constexpr int kHalves = D / 128;
+  static constexpr uint32_t kGroupBytes = D / 8 * 128;                // eight keys
+  static constexpr int kSmem = 1024 + (kKBufs + kVBufs) * kTileBytes + 4 * kRawBytes;
+};
+
+struct TcShared {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, s_read, p_full, o_full, o_read;
+  uint32_t tmem;
+  int bad;
+  uint32_t used[kTreeWords];               // rows of the tree that are used
+  uint32_t path[kTreeRows][kTreeWords + 1];  // what each row sees of the tree
+  int parents[kTreeRows];
+  float scale[kScaleBufs][3][kTcKeys];      // keys', values', log2 of the latter's magnitude
+  float top[2][2][kTcRows][2];              // [tile & 1][half of the keys][row]: largest score, largest score + log2 scale
+  float q_most[2][kTcRows];
+  float sum[2][kTcRows];
+};
+
+__device__ __forceinline__ void tc_alloc(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_free(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+// D (tensor memory) [+]= A (tensor memory) B (shared memory)
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{.reg .pred p; setp.ne.b32 p, %4, 0; "
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_load32(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+      "%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tc_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void to_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Operand B without swizzle: core matrices of eight rows of 16 bytes; `lead` and `stride`: bytes between core matrices.  Keys
+// (elements along head_dim contract): lead along head_dim, stride along the keys.  Values (keys contract, head_dim runs within a
+// core matrix' rows): lead along the keys, stride along head_dim.
+__device__ __forceinline__ uint64_t tc_operand(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | static_cast<uint64_t>((lead >> 4) & 0x3FFF) << 16 |
+         static_cast<uint64_t>((stride >> 4) & 0x3FFF) << 32 | 1ull << 46;
+}
+// fp32 results of binary16 operands, 128 rows, n columns; turned: B's rows are the contracted index
+__device__ __forceinline__ uint32_t tc_shape(uint32_t n, bool turned) {
+  return (1u << 4) | (turned ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((kTcRows >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t tree_pack(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ void tree_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = tree_pack(h);
+  lo = tree_pack(__floats2half2_rn(x - f.x, y - f.y));
+}
+// The same of the products x u and y v, with one rounding.
+__device__ __forceinline__ void tree_split_product(float x, float y, float u, float v, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x * u, y * v);
+  const float2 f = __half22float2(h);
+  hi = tree_pack(h);
+  lo = tree_pack(__floats2half2_rn(fmaf(x, u, -f.x), fmaf(y, v, -f.y)));
+}
+// Bits [a, b) of a word, a and b anything.
+__device__ __forceinline__ uint32_t bits_between(int a, int b) {
+  a = max(a, 0), b = min(b, 32);
+  return a >= b ? 0u : (0xFFFFFFFFu >> (32 - (b - a))) << a;
+}
+
+// Four cache elements of a 32-bit word (eight of 4 bits) as binary16; true where one is not finite.
 template <int KV>
-int launch_tree(const TreeParams& p, uint64_t head_dim, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(p.heads), static_cast<unsigned>(p.m));
-  if (head_dim == 256) attention_tree_rows_kernel<KV, 256><<<grid, kTreeWarps * 32, 0, st>>>(p);
-  else attention_tree_rows_kernel<KV, 128><<<grid, kTreeWarps * 32, 0, st>>>(p);
+__device__ __forceinline__ bool tree_expand(uint32_t w, uint32_t (&h)[KV == kKvInt4 ? 4 : 2]) {
+  auto minus = [](uint32_t a, uint32_t b) { return tree_pack(__hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b))); };
+  if constexpr (KV == kKvFp8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      h[i] = tree_pack(__half2(__half2_raw(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w >> (16 * i)) & 0xFFFFu), __NV_E4M3))));
+    return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+  } else if constexpr (KV == kKvInt8) {  // 1024 + (b + 128) - 1152, exact
+    const uint32_t u = w ^ 0x80808080u;
+    h[0] = minus(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);
+    h[1] = minus(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u);
+    return false;
+  } else {  // two's-complement nibbles, element 2i low: 1024 + (v + 8) - 1032
+    const uint32_t t = w ^ 0x88888888u, even = t & 0x0F0F0F0Fu, odd = (t >> 4) & 0x0F0F0F0Fu;
+    const uint32_t x = __byte_perm(even, odd, 0x5140), y = __byte_perm(even, odd, 0x7362);
+    h[0] = minus(__byte_perm(x, 0x64646464u, 0x4140), 0x64086408u);
+    h[1] = minus(__byte_perm(x, 0x64646464u, 0x4342), 0x64086408u);
+    h[2] = minus(__byte_perm(y, 0x64646464u, 0x4140), 0x64086408u);
+    h[3] = minus(__byte_perm(y, 0x64646464u, 0x4342), 0x64086408u);
+    return false;
+  }
+}
+__device__ __forceinline__ bool halves_not_finite(uint32_t w) { return (((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0; }
+
+// Every row's path: pointer doubling, a thread a row of the tree; then the window.  All threads of the CTA.
+__device__ __forceinline__ void tree_paths(TcShared& sh, int m, int window) {
+  const int i = threadIdx.x;
+  int up = -2;
+  uint32_t mine[kTreeWords];
+  if (i < m) {
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) sh.path[i][w] = mine[w] = w == i >> 5 ? 1u << (i & 31) : 0u;
+    sh.path[i][kTreeWords] = 0;
+    const int p = sh.parents[i];
+    up = p < -1 || p >= i ? -2 : p;
+  }
+  __syncthreads();
+  if (i < m) sh.parents[i] = up;
+  while (__syncthreads_or(up >= 0)) {
+    int next = up;
+    if (up >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) mine[w] |= sh.path[up][w];
+      next = sh.parents[up];
+    }
+    __syncthreads();
+    if (up >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) sh.path[i][w] = mine[w];
+      sh.parents[i] = next;
+    }
+    up = next;
+  }
+  if (i < m) {
+    int length = 0;
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) {
+      if (up != -1) mine[w] = 0;
+      length += __popc(mine[w]);
+    }
+    if (length != 0) atomicOr(&sh.used[i >> 5], 1u << (i & 31));
+    if (window != 0) {  // the nearest ancestors have the highest bits
+      int over = length - window;
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) {
+        const int here = __popc(mine[w]);
+        if (over >= here) mine[w] = 0;
+        else
+          for (int x = 0; x < over; ++x) mine[w] &= mine[w] - 1;
+        over -= here;
+        if (over < 0) over = 0;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) sh.path[i][w] = mine[w];
+  }
+  __syncthreads();
+}
+
+// Rows [0, rows) of the CTA over keys [c0, c1), a warp a row and key by key in fp32: where something is not finite.
+template <int KV, int D>
+__device__ __noinline__ void tree_scalar_rows(const TcParams& p, const TcShared& sh, int kv, int row0, int rows, int c0, int c1, int split) {
+  constexpr bool kScaled = KV >= kKvFp8;
+  constexpr size_t kRowBytes = static_cast<size_t>(D) * kv_bits<KV>() / 8;
+  const int lane = threadIdx.x & 31, n = p.t.n;
+  const size_t row_bytes = p.t.kv_heads * kRowBytes;
+  for (int r = threadIdx.x >> 5; r < rows; r += kSoftThreads / 32) {
+    const int i = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - i * p.group;
+    int length = 0;
+    for (int w = 0; w < kTreeWords; ++w) length += __popc(sh.path[i][w]);
+    const int first = length == 0 ? n : p.t.window != 0 ? max(0, n - (p.t.window - length)) : 0;
+    const size_t at = (static_cast<size_t>(i) * p.t.heads + h) * D;
+    float x[D / 32], acc[D / 32], top = kNoKey, total = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) x[e] = p.t.q[at + e * 32 + lane] * (kLog2e / sqrtf(static_cast<float>(D))), acc[e] = 0.0f;
+    for (int j = max(first, c0); j < c1; ++j) {
+      if (j >= n && !(sh.path[i][(j - n) >> 5] >> ((j - n) & 31) & 1u)) continue;
+      const unsigned char *kr = p.t.k + j * row_bytes + kv * kRowBytes, *vr = p.t.v + j * row_bytes + kv * kRowBytes;
+      float dot = 0.0f;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) dot = fmaf(x[e], tree_element<KV>(kr, e * 32 + lane), dot);
+      const float sc = warp_sum(dot) * (kScaled ? p.t.ks[j] : 1.0f), now = fmaxf(top, sc);
+      const float corr = exp2f(top - now), w = exp2f(sc - now), wv = w * (kScaled ? p.t.vs[j] : 1.0f);
+      total = fmaf(total, corr, w);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wv, tree_element<KV>(vr, e * 32 + lane), acc[e] * corr);
+      top = now;
+    }
+    const size_t part = (static_cast<size_t>(i) * p.t.heads + h) * p.splits + split;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      if (p.pacc != nullptr) p.pacc[part * D + e * 32 + lane] = acc[e];
+      else p.t.out[at + e * 32 + lane] = total == 0.0f ? 0.0f : acc[e] / total;
+    }
+    if (p.pacc != nullptr && lane == 0) p.pmax[part] = top, p.psum[part] = total;
+  }
+}
+
+// The loading warps' part: tile t of the keys (VALUES: of the values) into its operand buffer, raw bytes from `raw`.
+template <int KV, int D>
+struct TcLoader {
+  using S = TcShape<KV, D>;
+  const TcParams& p;
+  TcShared& sh;
+  int kv, c0, c1, tiles;
+
+  __device__ __forceinline__ const unsigned char* base(bool values) const {
+    return (values ? p.t.v : p.t.k) + static_cast<size_t>(kv) * S::kRowBytes;
+  }
+  __device__ __forceinline__ size_t pitch() const { return static_cast<size_t>(p.t.kv_heads) * S::kRowBytes; }
+  // whether key j is a row of the tree that nobody sees: read as zeros
+  __device__ __forceinline__ bool unseen(int j) const {
+    const int i = j - p.t.n;
+    return i >= 0 && !(sh.used[i >> 5] >> (i & 31) & 1u);
+  }
+  // 16-byte piece x of a tile: keys run fastest, eight at a time, so that stores to the operand's layout are conflict-free and a
+  // key's pieces of a warp are neighbours in memory
+  static __device__ __forceinline__ void piece(int x, int& key, int& c) {
+    constexpr int kC = S::kRowBytes / 16, kAtOnce = kC < 4 ? kC : 4;
+    const int lane = x % (8 * kAtOnce), rest = x / (8 * kAtOnce);
+    key = lane % 8 + 8 * (rest % (kTcKeys / 8));
+    c = lane / 8 + kAtOnce * (rest / (kTcKeys / 8));
+  }
+  __device__ __forceinline__ void fetch(bool values, int t, unsigned char* dst, int tid) const {  // raw bytes, or fp16 in place
+    if (t < tiles) {
+      for (int x = tid; x < kTcKeys * S::kRowBytes / 16; x += kLoadThreads) {
+        int key, c;
+        piece(x, key, c);
+        const int j = min(c0 + t * kTcKeys + key, c1 - 1);
+        const uint32_t at = KV == kKvF16 ? (key / 8) * S::kGroupBytes + (key % 8) * 16 + c * 128 : x * 16;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + at), "l"(base(values) + j * pitch() + c * 16) : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ bool convert(int t, const unsigned char* raw, unsigned char* dst, int tid) const {
+    bool bad = false;
+    for (int x = tid; x < kTcKeys * S::kRowBytes / 16; x += kLoadThreads) {
+      int key, c;
+      piece(x, key, c);
+      const bool zero = unseen(min(c0 + t * kTcKeys + key, c1 - 1));
+      if constexpr (KV == kKvF16) {
+        uint4* at = reinterpret_cast<uint4*>(dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + c * 128);
+        const uint4 y = *at;
+        if (zero) *at = make_uint4(0u, 0u, 0u, 0u);
+        else bad |= halves_not_finite(y.x) || halves_not_finite(y.y) || halves_not_finite(y.z) || halves_not_finite(y.w);
+      } else {
+        constexpr int kWords = KV == kKvInt4 ? 4 : 2;  // of 16 bytes of operand a piece becomes
+        uint4 y = *reinterpret_cast<const uint4*>(raw + x * 16);
+        if (zero) y = make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+        uint32_t h[4][KV == kKvInt4 ? 4 : 2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= tree_expand<KV>(w[i], h[i]);
+#pragma unroll
+        for (int o = 0; o < kWords; ++o) {
+          const uint4 z = KV == kKvInt4 ? make_uint4(h[o][0], h[o][1], h[o][2 % kWords], h[o][3 % kWords])
+                                        : make_uint4(h[2 * (o & 1)][0], h[2 * (o & 1)][1], h[2 * (o & 1) + 1][0], h[2 * (o & 1) + 1][1]);
+          *reinterpret_cast<uint4*>(dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + (c * kWords + o) * 128) = z;
+        }
+      }
+    }
+    return bad;
+  }
+  // fp32 rows, a warp each: scaled by a power of two to [2^13, 2^14), two terms
+  __device__ __forceinline__ bool split_rows(bool values, int t, unsigned char* dst, int tid) const {
+    constexpr int kLoadWarps = kLoadThreads / 32, kRun = 512 / D, kPer = D / 128;
+    const int lane = tid & 31, warp = tid >> 5;
+    bool bad = false;
+    for (int k0 = warp; k0 < kTcKeys; k0 += kLoadWarps * kRun) {
+      float4 x[kRun][kPer];
+#pragma unroll
+      for (int u = 0; u < kRun; ++u) {
+        const int key = k0 + u * kLoadWarps, j = min(c0 + t * kTcKeys + key, c1 - 1);
+        const float4* src = reinterpret_cast<const float4*>(base(values) + j * pitch()) + lane;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[u][i] = key < kTcKeys && !unseen(j) ? __ldg(src + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < kRun; ++u) {
+        const int key = k0 + u * kLoadWarps;
+        if (key >= kTcKeys) break;
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          most = max(max(most, max(__float_as_uint(x[u][i].x) & 0x7FFFFFFFu, __float_as_uint(x[u][i].y) & 0x7FFFFFFFu)),
+                     max(__float_as_uint(x[u][i].z) & 0x7FFFFFFFu, __float_as_uint(x[u][i].w) & 0x7FFFFFFFu));
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
+        bad |= most >= 0x7F800000u;
+        const int e = most == 0 ? 0 : max(-110, min(114, static_cast<int>(most >> 23) - 127 - 13));
+        const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        if (lane == 0) {
+          float* sc = &sh.scale[t % kScaleBufs][values ? 1 : 0][key];
+          sc[0] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+          if (values) sc[kTcKeys] = static_cast<float>(e);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          uint2 hi, lo;
+          tree_split(x[u][i].x * up, x[u][i].y * up, hi.x, lo.x);
+          tree_split(x[u][i].z * up, x[u][i].w * up, hi.y, lo.y);
+          const int c = i * 16 + lane / 2;
+          unsigned char* at = dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + c * 128 + (lane & 1) * 8;
+          *reinterpret_cast<uint2*>(at) = hi;
+          *reinterpret_cast<uint2*>(at + S::kTermBytes) = lo;
+        }
+      }
+    }
+    return bad;
+  }
+  // a quantised tile's scales: asked for a tile ahead, put where the weights are formed
+  __device__ __forceinline__ void next_scales(int t, int tid, float& k, float& v) const {
+    k = v = 0.0f;
+    if (tid >= kTcKeys || t >= tiles) return;
+    const int j = min(c0 + t * kTcKeys + tid, c1 - 1);
+    if (!unseen(j)) k = __ldg(p.t.ks + j), v = __ldg(p.t.vs + j);
+  }
+  __device__ __forceinline__ bool put_scales(int t, int tid, float k, float v) const {
+    if (tid >= kTcKeys) return false;
+    float(*sc)[kTcKeys] = sh.scale[t % kScaleBufs];
+    sc[0][tid] = k, sc[1][tid] = v, sc[2][tid] = log2f(fabsf(v));
+    return !(fabsf(k) <= 3.402823466e38f) || !(fabsf(v) <= 3.402823466e38f);
+  }
+};
+
+template <int KV, int D>
+__global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const TcParams p) {
+  using S = TcShape<KV, D>;
+  constexpr bool kScaled = KV != kKvF16;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(16) TcShared sh;
+  unsigned char* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* const k_s = smem;                               // [kKBufs][terms][64 keys][D]
+  unsigned char* const v_s = k_s + S::kKBufs * S::kTileBytes;  // [kVBufs] ...
+  unsigned char* const raw_s = v_s + S::kVBufs * S::kTileBytes;  // [2][keys, values]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kv = blockIdx.x % p.t.kv_heads, row0 = static_cast<int>(blockIdx.x) / p.t.kv_heads * kTcRows, split = blockIdx.y;
+  const int rows = min(kTcRows, p.t.m * p.group - row0), n = p.t.n;
+  const int c0 = p.first_key + split * p.tiles_per_split * kTcKeys;
+  const int c1 = static_cast<int>(min(static_cast<long long>(n) + p.t.m, static_cast<long long>(c0) + static_cast<long long>(p.tiles_per_split) * kTcKeys));
+  const int tiles = (c1 - c0 + kTcKeys - 1) / kTcKeys;
+  const bool loading = warp >= kSoftThreads / 32 && warp < (kSoftThreads + kLoadThreads) / 32;
+  const int load_tid = tid - kSoftThreads;
+  TcLoader<KV, D> loader{p, sh, kv, c0, c1, tiles};
+
+  if (loading) {  // the first tiles are under way before anything else
+    if (S::kRaw) {
+      loader.fetch(false, 0, raw_s, load_tid), loader.fetch(true, 0, raw_s + S::kRawBytes, load_tid);
+      loader.fetch(false, 1, raw_s + 2 * S::kRawBytes, load_tid), loader.fetch(true, 1, raw_s + 3 * S::kRawBytes, load_tid);
+    } else if (KV == kKvF16) {
+      loader.fetch(false, 0, k_s, load_tid), loader.fetch(true, 0, v_s, load_tid);
+      loader.fetch(false, 1, k_s + S::kTileBytes, load_tid), loader.fetch(true, 1, v_s + S::kTileBytes, load_tid);
+    }
+  }
+  if (tid < kTreeWords) sh.used[tid] = 0;
+  if (tid < p.t.m) sh.parents[tid] = p.t.parents[tid];
+  if (tid == 0) {
+    sh.bad = 0;
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sh.k_full[b], kLoadThreads / 32), mbar_init(&sh.v_full[b], kLoadThreads / 32);
+      mbar_init(&sh.k_empty[b], 1), mbar_init(&sh.v_empty[b], 1);
+    }
+    mbar_init(&sh.s_full, 1), mbar_init(&sh.o_full, 1);
+    mbar_init(&sh.s_read, kSoftThreads / 32), mbar_init(&sh.p_full, kSoftThreads / 32), mbar_init(&sh.o_read, kSoftThreads / 32);
+    mbar_fence_init();
+  }
+  if (warp == kTcThreads / 32 - 1) tc_alloc(&sh.tmem);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  tree_paths(sh, p.t.m, p.t.window);
+  const uint32_t tmem = sh.tmem;
+  // a thread's row
+  const int half = warp >> 2, row = (warp & 3) * 32 + lane;  // (of warps 0-7)
+  const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+  const int tree_i = row < rows ? (row0 + row) / p.group : 0;
+  const int head = kv * p.group + (row0 + row) - tree_i * p.group;
+  float row_f = 0.0f;
+  int first = 0x7FFFFFFF;
+  if (warp < kSoftThreads / 32) {
+    // queries: scaled by a power of two to [2^13, 2^14), two terms, to tensor memory; a thread half a row
+    bool seeing = false;
+    if (row < rows) {
+      int length = 0;
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) length += __popc(sh.path[tree_i][w]);
+      seeing = length != 0;
+      if (seeing) first = p.t.window != 0 ? max(0, n - (p.t.window - length)) : 0;
+    }
+    const float4* src = reinterpret_cast<const float4*>(p.t.q + (static_cast<size_t>(tree_i) * p.t.heads + head) * D + half * (D / 2));
+    float4 x[D / 8];
+    float most = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) x[i] = seeing ? __ldg(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const float a = fmaxf(fabsf(x[i].x), fabsf(x[i].y)), b = fmaxf(fabsf(x[i].z), fabsf(x[i].w));
+      bad |= !(fabsf(x[i].x) <= 3.402823466e38f) || !(fabsf(x[i].y) <= 3.402823466e38f) || !(fabsf(x[i].z) <= 3.402823466e38f) ||
+             !(fabsf(x[i].w) <= 3.402823466e38f);
+      most = fmaxf(most, fmaxf(a, b));
+    }
+    if (bad) sh.bad = 1;
+    sh.q_most[half][row] = most;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    most = fmaxf(most, sh.q_most[half ^ 1][row]);
+    int e = static_cast<int>((__float_as_uint(most) >> 23) & 0xFFu) - 127 - 13;
+    e = most == 0.0f ? 0 : max(-110, min(114, e));
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    row_f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (kLog2e / sqrtf(static_cast<float>(D)));
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      uint32_t hi[16], lo[16];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float4 y = x[i * 8 + u];
+        tree_split(y.x * up, y.y * up, hi[2 * u], lo[2 * u]);
+        tree_split(y.z * up, y.w * up, hi[2 * u + 1], lo[2 * u + 1]);
+      }
+      tc_store16(tmem + lanes + kColQ + half * (D / 4) + i * 16, hi);
+      tc_store16(tmem + lanes + kColQ + D / 2 + half * (D / 4) + i * 16, lo);
+    }
+    tc_store_wait();
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+
+  // the softmax warps hold 128 sums a thread where head_dim is 256: 256 * 208 + 128 * 88 registers, the launch's 384 * 168
+  if (D == 256) {
+    if (warp < kSoftThreads / 32) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
+  // Once a wait has given up (counted, and told to the host) a thread waits no more and goes on to the end of its loop, so that
+  // everybody comes to the barriers.
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, int phase) {
+    if (ok) ok = mbar_wait(bar, phase & 1, &g_tree_timeouts);
+  };
+  if (warp < kSoftThreads / 32) {
+    float o[S::kHalves][64];
+#pragma unroll
+    for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+      for (int c = 0; c < 64; ++c) o[h][c] = 0.0f;
+    float mx = kNoKey, sum = 0.0f, unit = 0.0f;
+    // outputs of half h (the tile before last's maximum is theirs: scaled by `unit` and added)
+    auto take = [&](float (&acc)[64]) {
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint32_t y[32];
+        tc_load32(tmem + lanes + kColO + half * 64 + part * 32, y);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) acc[part * 32 + c] = fmaf(__uint_as_float(y[c]), unit, acc[part * 32 + c]);
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.o_read);
+    };
+    for (int t = 0; t < tiles; ++t) {
+      wait(&sh.s_full, t);
+      tc_after();
+      uint32_t s[32];
+      tc_load32(tmem + lanes + kColS + half * 32, s);
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.s_read);
+      if (KV == kKvF32) wait(&sh.v_full[t % S::kVBufs], t / S::kVBufs);  // (their scales come with the values)
+      // which of the 32 keys the row sees
+      const int j0 = c0 + t * kTcKeys + half * 32;
+      uint32_t see = 0xFFFFFFFFu;
+      if (j0 < first || j0 + 32 > n) {
+        see = first == 0x7FFFFFFF ? 0u : bits_between(first - j0, n - j0);
+        const int off = j0 - n;
+        if (off > -32 && row < rows) {
+          const uint32_t* path = sh.path[tree_i];
+          if (off < 0) see |= path[0] << -off;
+          else if (off < kTreeRows) see |= __funnelshift_r(path[off >> 5], path[(off >> 5) + 1], off & 31);
+        }
+      }
+      const float* ks = sh.scale[t % kScaleBufs][0] + half * 32;
+      const float* vs = sh.scale[t % kScaleBufs][1] + half * 32;
+      const float* lv = sh.scale[t % kScaleBufs][2] + half * 32;
+      float top = kNoKey, most = kNoKey;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        const float y = __uint_as_float(s[c]) * (kScaled ? row_f * ks[c] : row_f);
+        if (see >> c & 1u) {
+          top = fmaxf(top, y);
+          if (kScaled) most = fmaxf(most, y + lv[c]);
+        }
+      }
+      float(*ex)[kTcRows][2] = sh.top[t & 1];
+      *reinterpret_cast<float2*>(ex[half][row]) = make_float2(top, most);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const float2 other = *reinterpret_cast<const float2*>(ex[half ^ 1][row]);
+      const float now = fmaxf(mx, fmaxf(top, other.x));
+      most = kScaled ? fmaxf(most, other.y) : fmaxf(top, other.x);
+      const float corr = exp2f(mx - now);
+      mx = now;
+      sum *= corr;
+      // the power of two that takes the row's largest weight (times its value's scale) to (2^13, 2^14]
+      const int e = static_cast<int>(fminf(fmaxf(ceilf(most - now), -110.0f), 126.0f));
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e < 254 ? 127 + 14 - e : 254) << 23);
+      uint32_t hi[16], lo[16];
+      float part = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        float w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float x = fmaf(__uint_as_float(s[c + u]), kScaled ? row_f * ks[c + u] : row_f, -now);
+          w[u] = see >> (c + u) & 1u ? exp2f(fminf(x, 1.0f)) : 0.0f;
+          part += w[u];
+        }
+        if (kScaled) tree_split_product(w[0] * up, w[1] * up, vs[c], vs[c + 1], hi[c / 2], lo[c / 2]);
+        else tree_split(w[0] * up, w[1] * up, hi[c / 2], lo[c / 2]);
+      }
+      sum += part;
+      // the tile before: its second half (its only one where head_dim is 128) leaves the weights' columns free
+      if (t > 0) {
+        wait(&sh.o_full, S::kHalves * t - 1);
+        tc_after();
+        take(o[S::kHalves - 1]);
+      }
+      tc_store16(tmem + lanes + kColP + half * 16, hi);
+      tc_store16(tmem + lanes + kColP + 32 + half * 16, lo);
+      tc_store_wait();
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full);
+      if (__any_sync(0xFFFFFFFFu, corr != 1.0f)) {
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+          for (int c = 0; c < 64; ++c) o[h][c] *= corr;
+      }
+      unit = 1.0f / up;
+      if (S::kHalves == 2) {
+        wait(&sh.o_full, 2 * t);
+        tc_after();
+        take(o[0]);
+      }
+    }
+    wait(&sh.o_full, S::kHalves * tiles - 1);
+    tc_after();
+    take(o[S::kHalves - 1]);
+    sh.sum[half][row] = sum;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (sh.bad != 0) {
+      tree_scalar_rows<KV, D>(p, sh, kv, row0, rows, c0, c1, split);
+    } else if (row < rows) {
+      sum += sh.sum[half ^ 1][row];
+      const size_t at = static_cast<size_t>(tree_i) * p.t.heads + head;
+      float* dst = p.pacc != nullptr ? p.pacc + (at * p.splits + split) * D : p.t.out + at * D;
+      const float f = p.pacc != nullptr ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+      for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+        for (int c = 0; c < 64; c += 4)
+          *reinterpret_cast<float4*>(dst + h * 128 + half * 64 + c) = make_float4(o[h][c] * f, o[h][c + 1] * f, o[h][c + 2] * f, o[h][c + 3] * f);
+      if (p.pacc != nullptr && half == 0) p.pmax[at * p.splits + split] = mx, p.psum[at * p.splits + split] = sum;
+    }
+  } else if (loading) {
+    bool bad = false;
+    float k_next = 0.0f, v_next = 0.0f;  // the next tile's scales
+    if (S::kRaw) loader.next_scales(0, load_tid, k_next, v_next);
+    for (int t = 0; t < tiles; ++t) {
+      const int kb = t % S::kKBufs, k_use = t / S::kKBufs, vb = t % S::kVBufs, v_use = t / S::kVBufs;
+      unsigned char *const k_dst = k_s + kb * S::kTileBytes, *const v_dst = v_s + vb * S::kTileBytes;
+      unsigned char* const raw = raw_s + (t & 1) * 2 * S::kRawBytes;  // a thread reads the pieces that it fetched
+      // keys: the buffer is free once the scores that read it are there
+      if (KV != kKvF16 && k_use > 0) wait(&sh.k_empty[kb], k_use - 1);
+      if constexpr (KV == kKvF32) {
+        bad |= loader.split_rows(false, t, k_dst, load_tid);
+      } else {
+        if constexpr (S::kRaw) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        else asm volatile("cp.async.wait_group 2;" ::: "memory");
+        bad |= loader.convert(t, raw, k_dst, load_tid);
+        if constexpr (S::kRaw) {
+          bad |= loader.put_scales(t, load_tid, k_next, v_next);
+          loader.next_scales(t + 1, load_tid, k_next, v_next);
+          loader.fetch(false, t + 2, raw, load_tid);
+        }
+      }
+      if (bad) sh.bad = 1;
+      to_async_proxy();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.k_full[kb]);
+      // values: the buffer is free once the outputs that read it are there
+      if (KV != kKvF16 && v_use > 0) wait(&sh.v_empty[vb], v_use - 1);
+      if constexpr (KV == kKvF32) {
+        bad |= loader.split_rows(true, t, v_dst, load_tid);
+      } else {
+        if constexpr (S::kRaw) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        else asm volatile("cp.async.wait_group 1;" ::: "memory");
+        bad |= loader.convert(t, raw + S::kRawBytes, v_dst, load_tid);
+        if constexpr (S::kRaw) loader.fetch(true, t + 2, raw + S::kRawBytes, load_tid);
+      }
+      if (bad) sh.bad = 1;
+      to_async_proxy();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.v_full[vb]);
+      if constexpr (KV == kKvF16) {
+        // The next tile's values and the keys of the one after it, straight into their buffers.  (The values of this tile's
+        // buffer are in use until the scores of the next tile have been issued, for which its keys have to be published first.)
+        if (t > 0) {
+          if (t + 1 < tiles) wait(&sh.v_empty[vb ^ 1], (t - 1) / 2);
+          loader.fetch(true, t + 1, v_s + (vb ^ 1) * S::kTileBytes, load_tid);
+        } else {
+          asm volatile("cp.async.commit_group;" ::: "memory");  // (its values are under way already)
+        }
+        if (t + 2 < tiles) wait(&sh.k_empty[kb], k_use);
+        loader.fetch(false, t + 2, k_dst, load_tid);
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (lane == 0) {
+    const uint32_t s_shape = tc_shape(kTcKeys, false), o_shape = tc_shape(128, true);
+    auto scores = [&](int t) {
+      const uint32_t at = smem_u32(k_s + (t % S::kKBufs) * S::kTileBytes);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {  // the small products first
+        const uint64_t b = tc_operand(at + kk * 256, 128, S::kGroupBytes);
+        tc_mma(tmem + kColS, tmem + kColQ + D / 2 + kk * 8, b, s_shape, kk != 0);
+        if (S::kTerms == 2) tc_mma(tmem + kColS, tmem + kColQ + kk * 8, tc_operand(at + S::kTermBytes + kk * 256, 128, S::kGroupBytes), s_shape, 1);
+      }
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        tc_mma(tmem + kColS, tmem + kColQ + kk * 8, tc_operand(at + kk * 256, 128, S::kGroupBytes), s_shape, 1);
+      tc_commit(&sh.s_full);
+      tc_commit(&sh.k_empty[t % S::kKBufs]);
+    };
+    auto outputs = [&](int t, int h) {
+      const uint32_t at = smem_u32(v_s + (t % S::kVBufs) * S::kTileBytes) + h * 2048;
+#pragma unroll
+      for (int kk = 0; kk < kTcKeys / 16; ++kk) {
+        const uint64_t b = tc_operand(at + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128);
+        tc_mma(tmem + kColO, tmem + kColP + 32 + kk * 8, b, o_shape, kk != 0);
+        if (S::kTerms == 2) tc_mma(tmem + kColO, tmem + kColP + kk * 8, tc_operand(at + S::kTermBytes + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128), o_shape, 1);
+      }
+#pragma unroll
+      for (int kk = 0; kk < kTcKeys / 16; ++kk)
+        tc_mma(tmem + kColO, tmem + kColP + kk * 8, tc_operand(at + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128), o_shape, 1);
+      tc_commit(&sh.o_full);
+      if (h == S::kHalves - 1) tc_commit(&sh.v_empty[t % S::kVBufs]);
+    };
+    wait(&sh.k_full[0], 0);
+    tc_after();
+    if (ok) scores(0);
+    for (int t = 0; t < tiles && ok; ++t) {
+      // outputs of a half: the weights and values are there, and the half before has been read
+      wait(&sh.p_full, t);
+      wait(&sh.v_full[t % S::kVBufs], t / S::kVBufs);
+      if (t > 0) wait(&sh.o_read, S::kHalves * t - 1);
+      tc_after();
+      if (ok) outputs(t, 0);
+      if (t + 1 < tiles) {
+        wait(&sh.s_read, t);
+        wait(&sh.k_full[(t + 1) % S::kKBufs], (t + 1) / S::kKBufs);
+        tc_after();
+        if (ok) scores(t + 1);
+      }
+      if (S::kHalves == 2) {
+        wait(&sh.o_read, 2 * t);
+        tc_after();
+        if (ok) outputs(t, 1);
+      }
+    }
+  }
+  __syncwarp();
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == kTcThreads / 32 - 1) tc_free(tmem);
+}
+
+// The chunks of a (row, head), a thread four elements; zero where no chunk had a key.
+__global__ void __launch_bounds__(256)
+attention_tree_merge_kernel(const float* __restrict__ pacc, const float* __restrict__ pmax, const float* __restrict__ psum,
+                            float* __restrict__ out, int dim4, int splits, size_t total) {
+  const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (t >= total) return;
+  const size_t row = t / dim4, e = t - row * dim4, base = row * splits;
+  float top = kNoKey, den = 0.0f;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, pmax[base + s]);
+  float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float w = exp2f(pmax[base + s] - top);
+    const float4 x = reinterpret_cast<const float4*>(pacc)[(base + s) * dim4 + e];
+    den = fmaf(w, psum[base + s], den);
+    num.x = fmaf(w, x.x, num.x), num.y = fmaf(w, x.y, num.y), num.z = fmaf(w, x.z, num.z), num.w = fmaf(w, x.w, num.w);
+  }
+  const float f = den == 0.0f ? 0.0f : 1.0f / den;
+  reinterpret_cast<float4*>(out)[t] = make_float4(num.x * f, num.y * f, num.z * f, num.w * f);
+}
+
+template <int KV, int D>
+int launch_tree_tc(TcParams p, cudaStream_t st) {
+  using S = TcShape<KV, D>;
+  static_assert(S::kSmem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
+  const auto kernel = attention_tree_tc_kernel<KV, D>;
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+  const dim3 grid(static_cast<unsigned>(p.t.kv_heads * p.row_tiles), static_cast<unsigned>(p.splits));
+  kernel<<<grid, kTcThreads, S::kSmem, st>>>(p);
+  if (int rc = check_launch(); rc != kOk || p.pacc == nullptr) return rc;
+  const size_t total = static_cast<size_t>(p.t.m) * p.t.heads * D / 4;
+  attention_tree_merge_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, st>>>(p.pacc, p.pmax, p.psum, p.t.out, D / 4, p.splits, total);
   return check_launch();
 }
 
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <int KV>
+int launch_tree(const TreeParams& t, uint64_t head_dim, cudaStream_t st) {
+  if (!on16(t.q) || !on16(t.k) || !on16(t.v) || !on16(t.out)) {
+    const dim3 grid(static_cast<unsigned>(t.heads), static_cast<unsigned>(t.m));
+    if (head_dim == 256) attention_tree_rows_kernel<KV, 256><<<grid, kTreeWarps * 32, 0, st>>>(t);
+    else attention_tree_rows_kernel<KV, 128><<<grid, kTreeWarps * 32, 0, st>>>(t);
+    return check_launch();
+  }
+  TcParams p{};
+  p.t = t;
+  p.group = t.heads / t.kv_heads;
+  p.row_tiles = (t.m * p.group + kTcRows - 1) / kTcRows;
+  p.first_key = t.window != 0 && t.window < t.n ? t.n - t.window : 0;
+  const long keys = static_cast<long>(t.n) + t.m - p.first_key, tiles = (keys + kTcKeys - 1) / kTcKeys;
+  const long units = static_cast<long>(t.kv_heads) * p.row_tiles;
+  // Chunks of the key range: whole waves of one CTA a SM, a CTA's start counted as four tiles.
+  static const int sms = [] {
+    int dev = 0, v = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    return v > 0 ? v : 148;
+  }();
+  long best_splits = 1;
+  double best = 0.0;
+  for (long s = 1; s <= 64 && s <= tiles; ++s) {
+    const long per = (tiles + s - 1) / s;
+    if ((tiles + per - 1) / per != s) continue;
+    const double waves = static_cast<double>((units * s + sms - 1) / sms);
+    const double cost = waves * (per + 4.0) + (s > 1 ? 2.0 + 0.1 * s : 0.0);
+    if (s == 1 || cost < best) best = cost, best_splits = s;
+  }
+  p.splits = static_cast<int>(best_splits);
+  p.tiles_per_split = static_cast<int>((tiles + best_splits - 1) / best_splits);
+  if (p.splits > 1) {
+    const size_t parts = static_cast<size_t>(t.m) * t.heads * p.splits;
+    const size_t acc_bytes = parts * head_dim * 4, stat_bytes = (parts * 4 + 255) / 256 * 256;
+    unsigned char* scratch = stream_scratch(st, acc_bytes + 2 * stat_bytes, 5);
+    if (scratch != nullptr) {
+      p.pacc = reinterpret_cast<float*>(scratch);
+      p.pmax = reinterpret_cast<float*>(scratch + acc_bytes);
+      p.psum = reinterpret_cast<float*>(scratch + acc_bytes + stat_bytes);
+    } else {  // a capture before the first plain launch: no chunks
+      p.splits = 1;
+      p.tiles_per_split = static_cast<int>(tiles);
+    }
+  }
+  return head_dim == 256 ? launch_tree_tc<KV, 256>(p, st) : launch_tree_tc<KV, 128>(p, st);
+}
+
 }  // namespace
+
+int tree_wait_timeouts(unsigned int* count) {
+  return cudaMemcpyFromSymbol(count, g_tree_timeouts, sizeof(*count)) == cudaSuccess ? kOk : kDeviceError;
+}
+int tree_set_error_word(unsigned int* word) { return set_host_error_word(word); }
 
 int attention_tree(int kv_format, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                                   const int32_t* parents, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
