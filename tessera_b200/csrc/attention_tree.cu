@@ -136,6 +136,8 @@ constexpr int kSoftThreads = 256, kLoadThreads = 96, kTcThreads = kSoftThreads +
 constexpr int kTcRows = 128, kTcKeys = 64;
 constexpr uint32_t kColQ = 0, kColS = 256, kColP = 320, kColO = 384;  // of tensor memory
 constexpr int kScaleBufs = 4;
+constexpr int kNoExponent = -1000;
+constexpr int kWideScales = 16;  // exponents apart
 
 struct TcParams {
   TreeParams t;
@@ -159,14 +161,16 @@ struct TcShape {
 struct TcShared {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, s_read, p_full, o_full, o_read;
   uint32_t tmem;
-  int bad;
   uint32_t used[kTreeWords];               // rows of the tree that are used
   uint32_t path[kTreeRows][kTreeWords + 1];  // what each row sees of the tree
   int parents[kTreeRows];
-  float scale[kScaleBufs][3][kTcKeys];      // keys', values', log2 of the latter's magnitude
-  float top[2][2][kTcRows][2];              // [tile & 1][half of the keys][row]: largest score, largest score + log2 scale
+  alignas(16) float scale[kScaleBufs][2][kTcKeys];  // keys', values'; read four at a time
+  int range[kScaleBufs][kLoadThreads / 32][2];      // largest and smallest exponent of the values' scales
+  float top[2][2][kTcRows];                         // [tile & 1][half of the keys][row]: largest score
+  float weighed[2][kTcRows];                        // the same of score + log2 of the value's scale
   float q_most[2][kTcRows];
   float sum[2][kTcRows];
+  int bad[kTcRows], any_bad;                        // rows with something that is not finite
 };
 
 __device__ __forceinline__ void tc_alloc(uint32_t* slot) {
@@ -192,12 +196,12 @@ __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::befor
 __device__ __forceinline__ void tc_load32(uint32_t at, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
-      "%27,%28,%29,%30,%31}, [%32];"
+      "%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"  // (one statement: the registers are not the results before the wait)
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
         "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
         "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(at));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      : "r"(at)
+      : "memory");
 }
 __device__ __forceinline__ void tc_store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]),
@@ -239,20 +243,18 @@ __device__ __forceinline__ uint32_t bits_between(int a, int b) {
   return a >= b ? 0u : (0xFFFFFFFFu >> (32 - (b - a))) << a;
 }
 
-// Four cache elements of a 32-bit word (eight of 4 bits) as binary16; true where one is not finite.
+// Four cache elements of a 32-bit word (eight of 4 bits) as binary16.
 template <int KV>
-__device__ __forceinline__ bool tree_expand(uint32_t w, uint32_t (&h)[KV == kKvInt4 ? 4 : 2]) {
+__device__ __forceinline__ void tree_expand(uint32_t w, uint32_t (&h)[KV == kKvInt4 ? 4 : 2]) {
   auto minus = [](uint32_t a, uint32_t b) { return tree_pack(__hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b))); };
   if constexpr (KV == kKvFp8) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       h[i] = tree_pack(__half2(__half2_raw(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w >> (16 * i)) & 0xFFFFu), __NV_E4M3))));
-    return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
   } else if constexpr (KV == kKvInt8) {  // 1024 + (b + 128) - 1152, exact
     const uint32_t u = w ^ 0x80808080u;
     h[0] = minus(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);
     h[1] = minus(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u);
-    return false;
   } else {  // two's-complement nibbles, element 2i low: 1024 + (v + 8) - 1032
     const uint32_t t = w ^ 0x88888888u, even = t & 0x0F0F0F0Fu, odd = (t >> 4) & 0x0F0F0F0Fu;
     const uint32_t x = __byte_perm(even, odd, 0x5140), y = __byte_perm(even, odd, 0x7362);
@@ -260,10 +262,16 @@ __device__ __forceinline__ bool tree_expand(uint32_t w, uint32_t (&h)[KV == kKvI
     h[1] = minus(__byte_perm(x, 0x64646464u, 0x4342), 0x64086408u);
     h[2] = minus(__byte_perm(y, 0x64646464u, 0x4140), 0x64086408u);
     h[3] = minus(__byte_perm(y, 0x64646464u, 0x4342), 0x64086408u);
-    return false;
   }
 }
-__device__ __forceinline__ bool halves_not_finite(uint32_t w) { return (((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0; }
+// exp2 without the slow path for results below the normal numbers, which are 0
+__device__ __forceinline__ float tree_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e, e in [-126, 127]
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
 // Every row's path: pointer doubling, a thread a row of the tree; then the window.  All threads of the CTA.
 __device__ __forceinline__ void tree_paths(TcShared& sh, int m, int window) {
@@ -320,7 +328,7 @@ __device__ __forceinline__ void tree_paths(TcShared& sh, int m, int window) {
   __syncthreads();
 }
 
-// Rows [0, rows) of the CTA over keys [c0, c1), a warp a row and key by key in fp32: where something is not finite.
+// The marked rows of the CTA over keys [c0, c1), a warp a row and key by key in fp32: where something is not finite.
 template <int KV, int D>
 __device__ __noinline__ void tree_scalar_rows(const TcParams& p, const TcShared& sh, int kv, int row0, int rows, int c0, int c1, int split) {
   constexpr bool kScaled = KV >= kKvFp8;
@@ -328,6 +336,7 @@ __device__ __noinline__ void tree_scalar_rows(const TcParams& p, const TcShared&
   const int lane = threadIdx.x & 31, n = p.t.n;
   const size_t row_bytes = p.t.kv_heads * kRowBytes;
   for (int r = threadIdx.x >> 5; r < rows; r += kSoftThreads / 32) {
+    if (sh.bad[r] == 0) continue;
     const int i = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - i * p.group;
     int length = 0;
     for (int w = 0; w < kTreeWords; ++w) length += __popc(sh.path[i][w]);
@@ -376,60 +385,62 @@ struct TcLoader {
     const int i = j - p.t.n;
     return i >= 0 && !(sh.used[i >> 5] >> (i & 31) & 1u);
   }
-  // 16-byte piece x of a tile: keys run fastest, eight at a time, so that stores to the operand's layout are conflict-free and a
-  // key's pieces of a warp are neighbours in memory
-  static __device__ __forceinline__ void piece(int x, int& key, int& c) {
-    constexpr int kC = S::kRowBytes / 16, kAtOnce = kC < 4 ? kC : 4;
-    const int lane = x % (8 * kAtOnce), rest = x / (8 * kAtOnce);
-    key = lane % 8 + 8 * (rest % (kTcKeys / 8));
-    c = lane / 8 + kAtOnce * (rest / (kTcKeys / 8));
-  }
+  // A warp takes 16-byte pieces of a tile four neighbours of eight keys at a time, so that its stores to the operand's layout are
+  // conflict-free and it reads 64 bytes of a key side by side.  Piece `it` of a thread:
+  static constexpr int kTimes = kTcKeys * S::kRowBytes / 512;
+  static __device__ __forceinline__ int key_of(int it, int lane) { return (it & 7) * 8 + (lane & 7); }
+  static __device__ __forceinline__ int piece_of(int it, int lane) { return (it >> 3) * 4 + (lane >> 3); }
+  static __device__ __forceinline__ uint32_t operand_at(int it, int lane, int c) { return (it & 7) * S::kGroupBytes + (lane & 7) * 16 + c * 128; }
   __device__ __forceinline__ void fetch(bool values, int t, unsigned char* dst, int tid) const {  // raw bytes, or fp16 in place
     if (t < tiles) {
-      for (int x = tid; x < kTcKeys * S::kRowBytes / 16; x += kLoadThreads) {
-        int key, c;
-        piece(x, key, c);
-        const int j = min(c0 + t * kTcKeys + key, c1 - 1);
-        const uint32_t at = KV == kKvF16 ? (key / 8) * S::kGroupBytes + (key % 8) * 16 + c * 128 : x * 16;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + at), "l"(base(values) + j * pitch() + c * 16) : "memory");
+      const int warp = tid >> 5, lane = tid & 31, j0 = c0 + t * kTcKeys;
+      const unsigned char* src = base(values) + static_cast<size_t>(j0) * pitch();
+      const int last = c1 - 1 - j0;
+      const uint32_t step = static_cast<uint32_t>(pitch());
+#pragma unroll 4
+      for (int it = warp; it < kTimes; it += kLoadThreads / 32) {
+        const int c = piece_of(it, lane);
+        const uint32_t at = KV == kKvF16 ? operand_at(it, lane, c) : it * 512 + lane * 16;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + at),
+                     "l"(src + static_cast<size_t>(min(key_of(it, lane), last)) * step + c * 16)
+                     : "memory");
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  __device__ __forceinline__ bool convert(int t, const unsigned char* raw, unsigned char* dst, int tid) const {
-    bool bad = false;
-    for (int x = tid; x < kTcKeys * S::kRowBytes / 16; x += kLoadThreads) {
-      int key, c;
-      piece(x, key, c);
-      const bool zero = unseen(min(c0 + t * kTcKeys + key, c1 - 1));
+  // Rows of the tree that nobody sees are zeros: what they hold may be anything.
+  __device__ __forceinline__ void convert(int t, const unsigned char* raw, unsigned char* dst, int tid) const {
+    const int warp = tid >> 5, lane = tid & 31, j0 = c0 + t * kTcKeys;
+    const bool past = j0 + kTcKeys <= p.t.n;
+    if (KV == kKvF16 && past) return;
+#pragma unroll 4
+    for (int it = warp; it < kTimes; it += kLoadThreads / 32) {
+      const int c = piece_of(it, lane);
+      const bool zero = !past && unseen(min(j0 + key_of(it, lane), c1 - 1));
       if constexpr (KV == kKvF16) {
-        uint4* at = reinterpret_cast<uint4*>(dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + c * 128);
-        const uint4 y = *at;
-        if (zero) *at = make_uint4(0u, 0u, 0u, 0u);
-        else bad |= halves_not_finite(y.x) || halves_not_finite(y.y) || halves_not_finite(y.z) || halves_not_finite(y.w);
+        if (zero) *reinterpret_cast<uint4*>(dst + operand_at(it, lane, c)) = make_uint4(0u, 0u, 0u, 0u);
       } else {
         constexpr int kWords = KV == kKvInt4 ? 4 : 2;  // of 16 bytes of operand a piece becomes
-        uint4 y = *reinterpret_cast<const uint4*>(raw + x * 16);
+        uint4 y = *reinterpret_cast<const uint4*>(raw + it * 512 + lane * 16);
         if (zero) y = make_uint4(0u, 0u, 0u, 0u);
         const uint32_t w[4] = {y.x, y.y, y.z, y.w};
         uint32_t h[4][KV == kKvInt4 ? 4 : 2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= tree_expand<KV>(w[i], h[i]);
+        for (int i = 0; i < 4; ++i) tree_expand<KV>(w[i], h[i]);
 #pragma unroll
         for (int o = 0; o < kWords; ++o) {
           const uint4 z = KV == kKvInt4 ? make_uint4(h[o][0], h[o][1], h[o][2 % kWords], h[o][3 % kWords])
                                         : make_uint4(h[2 * (o & 1)][0], h[2 * (o & 1)][1], h[2 * (o & 1) + 1][0], h[2 * (o & 1) + 1][1]);
-          *reinterpret_cast<uint4*>(dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + (c * kWords + o) * 128) = z;
+          *reinterpret_cast<uint4*>(dst + operand_at(it, lane, c * kWords + o)) = z;
         }
       }
     }
-    return bad;
   }
   // fp32 rows, a warp each: scaled by a power of two to [2^13, 2^14), two terms
-  __device__ __forceinline__ bool split_rows(bool values, int t, unsigned char* dst, int tid) const {
+  __device__ __forceinline__ void split_rows(bool values, int t, unsigned char* dst, int tid) const {
     constexpr int kLoadWarps = kLoadThreads / 32, kRun = 512 / D, kPer = D / 128;
     const int lane = tid & 31, warp = tid >> 5;
-    bool bad = false;
+    int high = kNoExponent, low = -kNoExponent;
     for (int k0 = warp; k0 < kTcKeys; k0 += kLoadWarps * kRun) {
       float4 x[kRun][kPer];
 #pragma unroll
@@ -449,14 +460,10 @@ struct TcLoader {
           most = max(max(most, max(__float_as_uint(x[u][i].x) & 0x7FFFFFFFu, __float_as_uint(x[u][i].y) & 0x7FFFFFFFu)),
                      max(__float_as_uint(x[u][i].z) & 0x7FFFFFFFu, __float_as_uint(x[u][i].w) & 0x7FFFFFFFu));
         most = __reduce_max_sync(0xFFFFFFFFu, most);
-        bad |= most >= 0x7F800000u;
         const int e = most == 0 ? 0 : max(-110, min(114, static_cast<int>(most >> 23) - 127 - 13));
-        const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        if (lane == 0) {
-          float* sc = &sh.scale[t % kScaleBufs][values ? 1 : 0][key];
-          sc[0] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-          if (values) sc[kTcKeys] = static_cast<float>(e);
-        }
+        const float up = power_of_two(-e);
+        if (most != 0) high = max(high, e), low = min(low, e);
+        if (lane == 0) sh.scale[t % kScaleBufs][values ? 1 : 0][key] = power_of_two(e);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           uint2 hi, lo;
@@ -469,7 +476,7 @@ struct TcLoader {
         }
       }
     }
-    return bad;
+    if (values && lane == 0) sh.range[t % kScaleBufs][warp][0] = high, sh.range[t % kScaleBufs][warp][1] = low;
   }
   // a quantised tile's scales: asked for a tile ahead, put where the weights are formed
   __device__ __forceinline__ void next_scales(int t, int tid, float& k, float& v) const {
@@ -478,11 +485,12 @@ struct TcLoader {
     const int j = min(c0 + t * kTcKeys + tid, c1 - 1);
     if (!unseen(j)) k = __ldg(p.t.ks + j), v = __ldg(p.t.vs + j);
   }
-  __device__ __forceinline__ bool put_scales(int t, int tid, float k, float v) const {
-    if (tid >= kTcKeys) return false;
-    float(*sc)[kTcKeys] = sh.scale[t % kScaleBufs];
-    sc[0][tid] = k, sc[1][tid] = v, sc[2][tid] = log2f(fabsf(v));
-    return !(fabsf(k) <= 3.402823466e38f) || !(fabsf(v) <= 3.402823466e38f);
+  __device__ __forceinline__ void put_scales(int t, int tid, float k, float v) const {
+    const uint32_t bits = __float_as_uint(v) & 0x7FFFFFFFu;
+    const int e = static_cast<int>(bits >> 23) - 126;  // |v| < 2^e
+    const int high = __reduce_max_sync(0xFFFFFFFFu, bits != 0 ? e : kNoExponent), low = __reduce_min_sync(0xFFFFFFFFu, bits != 0 ? e : -kNoExponent);
+    if ((tid & 31) == 0) sh.range[t % kScaleBufs][tid >> 5][0] = high, sh.range[t % kScaleBufs][tid >> 5][1] = low;
+    if (tid < kTcKeys) sh.scale[t % kScaleBufs][0][tid] = k, sh.scale[t % kScaleBufs][1][tid] = v;
   }
 };
 
@@ -516,9 +524,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     }
   }
   if (tid < kTreeWords) sh.used[tid] = 0;
+  if (tid < kTcRows) sh.bad[tid] = 0;
   if (tid < p.t.m) sh.parents[tid] = p.t.parents[tid];
   if (tid == 0) {
-    sh.bad = 0;
+    sh.any_bad = 0;
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.k_full[b], kLoadThreads / 32), mbar_init(&sh.v_full[b], kLoadThreads / 32);
       mbar_init(&sh.k_empty[b], 1), mbar_init(&sh.v_empty[b], 1);
@@ -553,24 +562,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     const float4* src = reinterpret_cast<const float4*>(p.t.q + (static_cast<size_t>(tree_i) * p.t.heads + head) * D + half * (D / 2));
     float4 x[D / 8];
     float most = 0.0f;
-    bool bad = false;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) x[i] = seeing ? __ldg(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
       const float a = fmaxf(fabsf(x[i].x), fabsf(x[i].y)), b = fmaxf(fabsf(x[i].z), fabsf(x[i].w));
-      bad |= !(fabsf(x[i].x) <= 3.402823466e38f) || !(fabsf(x[i].y) <= 3.402823466e38f) || !(fabsf(x[i].z) <= 3.402823466e38f) ||
-             !(fabsf(x[i].w) <= 3.402823466e38f);
       most = fmaxf(most, fmaxf(a, b));
     }
-    if (bad) sh.bad = 1;
     sh.q_most[half][row] = most;
     asm volatile("bar.sync 1, 256;" ::: "memory");
     most = fmaxf(most, sh.q_most[half ^ 1][row]);
     int e = static_cast<int>((__float_as_uint(most) >> 23) & 0xFFu) - 127 - 13;
     e = most == 0.0f ? 0 : max(-110, min(114, e));
-    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    row_f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (kLog2e / sqrtf(static_cast<float>(D)));
+    const float up = power_of_two(-e);
+    row_f = power_of_two(e) * (kLog2e / sqrtf(static_cast<float>(D)));
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       uint32_t hi[16], lo[16];
@@ -606,8 +611,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
       for (int c = 0; c < 64; ++c) o[h][c] = 0.0f;
-    float mx = kNoKey, sum = 0.0f, unit = 0.0f;
-    // outputs of half h (the tile before last's maximum is theirs: scaled by `unit` and added)
+    float mx = kNoKey, sum = 0.0f, unit = 0.0f;  // mx: a whole number, so that everything is rescaled by powers of two
+    // half of a tile's outputs, relative to the maximum when its weights were formed
     auto take = [&](float (&acc)[64]) {
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
@@ -643,43 +648,75 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       }
       const float* ks = sh.scale[t % kScaleBufs][0] + half * 32;
       const float* vs = sh.scale[t % kScaleBufs][1] + half * 32;
-      const float* lv = sh.scale[t % kScaleBufs][2] + half * 32;
-      float top = kNoKey, most = kNoKey;
+      // scores over row_f, -infinity for a key that the row does not see
+      if constexpr (kScaled) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const float y = __uint_as_float(s[c]) * (kScaled ? row_f * ks[c] : row_f);
-        if (see >> c & 1u) {
-          top = fmaxf(top, y);
-          if (kScaled) most = fmaxf(most, y + lv[c]);
+        for (int c = 0; c < 32; c += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(ks + c);
+          const float y[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[c + u] = __float_as_uint(__uint_as_float(s[c + u]) * y[u]);
         }
       }
-      float(*ex)[kTcRows][2] = sh.top[t & 1];
-      *reinterpret_cast<float2*>(ex[half][row]) = make_float2(top, most);
+      if (__any_sync(0xFFFFFFFFu, see != 0xFFFFFFFFu)) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          if (!(see >> c & 1u)) s[c] = 0xFF800000u;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(s[c]));
+      sh.top[t & 1][half][row] = top;
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const float2 other = *reinterpret_cast<const float2*>(ex[half ^ 1][row]);
-      const float now = fmaxf(mx, fmaxf(top, other.x));
-      most = kScaled ? fmaxf(most, other.y) : fmaxf(top, other.x);
-      const float corr = exp2f(mx - now);
+      top = fmaxf(top, sh.top[t & 1][half ^ 1][row]);
+      const float now = fmaxf(mx, ceilf(top * row_f));
+      const float corr = tree_exp2(mx - now);  // 1 while the row has had no key (kNoKey - kNoKey)
       mx = now;
-      sum *= corr;
-      // the power of two that takes the row's largest weight (times its value's scale) to (2^13, 2^14]
-      const int e = static_cast<int>(fminf(fmaxf(ceilf(most - now), -110.0f), 126.0f));
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e < 254 ? 127 + 14 - e : 254) << 23);
-      uint32_t hi[16], lo[16];
-      float part = 0.0f;
+      // The power of two that takes weights (at most 1) times their values' scales to at most 2^14.  What binary16 cuts off is 2^-39
+      // of that, so one for all keys will do while their scales lie within 2^16; else each row's is made for its largest.
+      int e = 0;
+      if (kScaled) {
+        const int(*range)[2] = sh.range[t % kScaleBufs];
+        int high = range[0][0], low = range[0][1];
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        float w[2];
+        for (int w = 1; w < kLoadThreads / 32; ++w) high = max(high, range[w][0]), low = min(low, range[w][1]);
+        e = high;
+        if (high - low > kWideScales) {
+          float most = kNoKey;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float x = fmaf(__uint_as_float(s[c + u]), kScaled ? row_f * ks[c + u] : row_f, -now);
-          w[u] = see >> (c + u) & 1u ? exp2f(fminf(x, 1.0f)) : 0.0f;
-          part += w[u];
+          for (int c = 0; c < 32; ++c) {
+            const uint32_t bits = __float_as_uint(vs[c]) & 0x7FFFFFFFu;
+            if (bits != 0) most = fmaxf(most, fmaf(__uint_as_float(s[c]), row_f, -now) + static_cast<float>(static_cast<int>(bits >> 23) - 126));
+          }
+          asm volatile("bar.sync 1, 256;" ::: "memory");  // (the tile before may still be reading)
+          sh.weighed[half][row] = most;
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          most = fmaxf(most, sh.weighed[half ^ 1][row]);
+          e = static_cast<int>(fminf(fmaxf(ceilf(most), -110.0f), 110.0f));
         }
-        if (kScaled) tree_split_product(w[0] * up, w[1] * up, vs[c], vs[c + 1], hi[c / 2], lo[c / 2]);
-        else tree_split(w[0] * up, w[1] * up, hi[c / 2], lo[c / 2]);
+        e = max(-110, min(110, e));
       }
-      sum += part;
+      const float shift = now == kNoKey ? 0.0f : static_cast<float>(14 - e) - now;
+      uint32_t hi[16], lo[16];
+      float part[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const float4 f = kScaled ? *reinterpret_cast<const float4*>(vs + c) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        const float y[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int u = 0; u < 4; u += 2) {
+          float w[2];
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            w[v] = tree_exp2(fmaf(__uint_as_float(s[c + u + v]), row_f, shift));
+            part[v] += w[v];
+          }
+          if (kScaled) tree_split_product(w[0], w[1], y[u], y[u + 1], hi[(c + u) / 2], lo[(c + u) / 2]);
+          else tree_split(w[0], w[1], hi[(c + u) / 2], lo[(c + u) / 2]);
+        }
+      }
+      const float next_unit = power_of_two(e - 14);
+      sum = fmaf(part[0] + part[1], next_unit, sum * corr);
       // the tile before: its second half (its only one where head_dim is 128) leaves the weights' columns free
       if (t > 0) {
         wait(&sh.o_full, S::kHalves * t - 1);
@@ -698,7 +735,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
 #pragma unroll
           for (int c = 0; c < 64; ++c) o[h][c] *= corr;
       }
-      unit = 1.0f / up;
+      unit = next_unit;
       if (S::kHalves == 2) {
         wait(&sh.o_full, 2 * t);
         tc_after();
@@ -708,11 +745,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     wait(&sh.o_full, S::kHalves * tiles - 1);
     tc_after();
     take(o[S::kHalves - 1]);
+    // A NaN or an infinity among a row's operands has made its sums so (that of a key which it does not see as well: its
+    // weight of 0 does not mask it).
+    float all = sum;
+#pragma unroll
+    for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+      for (int c = 0; c < 64; ++c) all = fmaf(o[h][c], 0.0f, all);
     sh.sum[half][row] = sum;
+    if (!(fabsf(all) <= 3.402823466e38f)) sh.bad[row] = sh.any_bad = 1;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (sh.bad != 0) {
-      tree_scalar_rows<KV, D>(p, sh, kv, row0, rows, c0, c1, split);
-    } else if (row < rows) {
+    if (sh.any_bad != 0) tree_scalar_rows<KV, D>(p, sh, kv, row0, rows, c0, c1, split);
+    if (row < rows && sh.bad[row] == 0) {
       sum += sh.sum[half ^ 1][row];
       const size_t at = static_cast<size_t>(tree_i) * p.t.heads + head;
       float* dst = p.pacc != nullptr ? p.pacc + (at * p.splits + split) * D : p.t.out + at * D;
@@ -725,7 +769,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       if (p.pacc != nullptr && half == 0) p.pmax[at * p.splits + split] = mx, p.psum[at * p.splits + split] = sum;
     }
   } else if (loading) {
-    bool bad = false;
     float k_next = 0.0f, v_next = 0.0f;  // the next tile's scales
     if (S::kRaw) loader.next_scales(0, load_tid, k_next, v_next);
     for (int t = 0; t < tiles; ++t) {
@@ -735,32 +778,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       // keys: the buffer is free once the scores that read it are there
       if (KV != kKvF16 && k_use > 0) wait(&sh.k_empty[kb], k_use - 1);
       if constexpr (KV == kKvF32) {
-        bad |= loader.split_rows(false, t, k_dst, load_tid);
+        loader.split_rows(false, t, k_dst, load_tid);
       } else {
         if constexpr (S::kRaw) asm volatile("cp.async.wait_group 3;" ::: "memory");
         else asm volatile("cp.async.wait_group 2;" ::: "memory");
-        bad |= loader.convert(t, raw, k_dst, load_tid);
+        loader.convert(t, raw, k_dst, load_tid);
         if constexpr (S::kRaw) {
-          bad |= loader.put_scales(t, load_tid, k_next, v_next);
+          loader.put_scales(t, load_tid, k_next, v_next);
           loader.next_scales(t + 1, load_tid, k_next, v_next);
           loader.fetch(false, t + 2, raw, load_tid);
         }
       }
-      if (bad) sh.bad = 1;
       to_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.k_full[kb]);
       // values: the buffer is free once the outputs that read it are there
       if (KV != kKvF16 && v_use > 0) wait(&sh.v_empty[vb], v_use - 1);
       if constexpr (KV == kKvF32) {
-        bad |= loader.split_rows(true, t, v_dst, load_tid);
+        loader.split_rows(true, t, v_dst, load_tid);
       } else {
         if constexpr (S::kRaw) asm volatile("cp.async.wait_group 3;" ::: "memory");
         else asm volatile("cp.async.wait_group 1;" ::: "memory");
-        bad |= loader.convert(t, raw + S::kRawBytes, v_dst, load_tid);
+        loader.convert(t, raw + S::kRawBytes, v_dst, load_tid);
         if constexpr (S::kRaw) loader.fetch(true, t + 2, raw + S::kRawBytes, load_tid);
       }
-      if (bad) sh.bad = 1;
       to_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.v_full[vb]);
