@@ -125,18 +125,18 @@ __global__ void __launch_bounds__(kTreeWarps * 32) attention_tree_rows_kernel(co
 // A CTA takes 128 (tree row, head) pairs of one kv head and walks over its share of the keys in tiles of 64, on tcgen05 binary16
 // MMAs with fp32 accumulators.  Cache elements are exact in binary16 (fp32 ones are two terms of a row scaled by a power of
 // two), a query element or a softmax weight is two terms, as in attention_tile.cu.  Everything the MMAs take from the left
-// lies in tensor memory: the queries' two terms for the whole call (an operand A in shared memory would be read again for every 64
-// columns, 48 cycles where the product takes 16), a tile's weights.  Columns of tensor memory: queries 256, scores 64, weights
-// 64, and 128 for the outputs of a tile, which are read after every tile -- half of head_dim at a time -- and added to
-// fp32 registers, so that what an accumulator cuts off does not add up over the keys.
+// lies in tensor memory: the queries' two terms for the whole call, a tile's weights over its scores.  Columns of tensor memory:
+// queries 256, two tiles' scores or weights 64 each, and 128 for the outputs of a tile, which are read after every tile -- half
+// of head_dim at a time -- and added to fp32 registers, so that what an accumulator cuts off does not add up over the keys.
 //   warps 0-7   a thread a row (tensor memory lane), warps 0-3 keys 0-31 of a tile and outputs 0-63 of a half, 4-7 the rest
 //   warps 8-10  keys and values: global memory -> binary16 in the operands' layout
-//   warp 11     one thread issues the MMAs: outputs' first half, the next scores, outputs' second half
+//   warp 11     one thread issues the MMAs: a tile's outputs, then the scores of the tile after next over its weights
 constexpr int kSoftThreads = 256, kLoadThreads = 96, kTcThreads = kSoftThreads + kLoadThreads + 32;
 constexpr int kTcRows = 128, kTcKeys = 64;
-constexpr uint32_t kColQ = 0, kColS = 256, kColP = 320, kColO = 384;  // of tensor memory
+constexpr uint32_t kColQ = 0, kColS = 256, kColO = 384;  // of tensor memory; tile t's scores and weights: kColS + 64 (t % 2)
 constexpr int kScaleBufs = 4;
 constexpr int kNoExponent = -1000;
+constexpr int kUnused = 0x7FFFFFFF;
 constexpr int kWideScales = 16;  // exponents apart
 
 struct TcParams {
@@ -158,8 +158,11 @@ struct TcShape {
   static constexpr int kSmem = 1024 + (kKBufs + kVBufs) * kTileBytes + 4 * kRawBytes;
 };
 
+// A parity wait tells a phase from the one before it, so no barrier may come two phases ahead of one who waits on it: scores and
+// weights have a barrier for either buffer, since the softmax warps give away a tile's weights before the MMAs have taken the
+// tile's before it; a phase of each other one is followed by the next only when everybody who waits for it has been heard of.
 struct TcShared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, s_read, p_full, o_full, o_read;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_read, drained;
   uint32_t tmem;
   uint32_t used[kTreeWords];               // rows of the tree that are used
   uint32_t path[kTreeRows][kTreeWords + 1];  // what each row sees of the tree
@@ -168,7 +171,8 @@ struct TcShared {
   int range[kScaleBufs][kLoadThreads / 32][2];      // largest and smallest exponent of the values' scales
   float top[2][2][kTcRows];                         // [tile & 1][half of the keys][row]: largest score
   float weighed[2][kTcRows];                        // the same of score + log2 of the value's scale
-  float q_most[2][kTcRows];
+  int first[kTcRows];                               // the first past row that a row sees (kUnused: it is not used)
+  float q_unit[kTcRows];
   float sum[2][kTcRows];
   int bad[kTcRows], any_bad;                        // rows with something that is not finite
 };
@@ -518,9 +522,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     if (S::kRaw) {
       loader.fetch(false, 0, raw_s, load_tid), loader.fetch(true, 0, raw_s + S::kRawBytes, load_tid);
       loader.fetch(false, 1, raw_s + 2 * S::kRawBytes, load_tid), loader.fetch(true, 1, raw_s + 3 * S::kRawBytes, load_tid);
-    } else if (KV == kKvF16) {
-      loader.fetch(false, 0, k_s, load_tid), loader.fetch(true, 0, v_s, load_tid);
-      loader.fetch(false, 1, k_s + S::kTileBytes, load_tid), loader.fetch(true, 1, v_s + S::kTileBytes, load_tid);
+    } else if (KV == kKvF16) {  // (the queries pass through the values' buffers first)
+      loader.fetch(false, 0, k_s, load_tid), loader.fetch(false, 1, k_s + S::kTileBytes, load_tid);
     }
   }
   if (tid < kTreeWords) sh.used[tid] = 0;
@@ -532,8 +535,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       mbar_init(&sh.k_full[b], kLoadThreads / 32), mbar_init(&sh.v_full[b], kLoadThreads / 32);
       mbar_init(&sh.k_empty[b], 1), mbar_init(&sh.v_empty[b], 1);
     }
-    mbar_init(&sh.s_full, 1), mbar_init(&sh.o_full, 1);
-    mbar_init(&sh.s_read, kSoftThreads / 32), mbar_init(&sh.p_full, kSoftThreads / 32), mbar_init(&sh.o_read, kSoftThreads / 32);
+    mbar_init(&sh.s_full[0], 1), mbar_init(&sh.s_full[1], 1), mbar_init(&sh.o_full, 1), mbar_init(&sh.drained, 1);
+    mbar_init(&sh.p_full[0], kSoftThreads / 32), mbar_init(&sh.p_full[1], kSoftThreads / 32), mbar_init(&sh.o_read, kSoftThreads / 32);
     mbar_fence_init();
   }
   if (warp == kTcThreads / 32 - 1) tc_alloc(&sh.tmem);
@@ -546,53 +549,79 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
   const int half = warp >> 2, row = (warp & 3) * 32 + lane;  // (of warps 0-7)
   const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
   const int tree_i = row < rows ? (row0 + row) / p.group : 0;
-  const int head = kv * p.group + (row0 + row) - tree_i * p.group;
   float row_f = 0.0f;
-  int first = 0x7FFFFFFF;
+  int first = kUnused;
   if (warp < kSoftThreads / 32) {
-    // queries: scaled by a power of two to [2^13, 2^14), two terms, to tensor memory; a thread half a row
-    bool seeing = false;
+    // Queries: a warp reads its sixteen rows whole, scales each by a power of two to [2^13, 2^14) and leaves it in shared memory
+    // (16-byte piece c of a row at c ^ (row & 7)) half a row after the other; a thread takes half a row of two terms to tensor memory.
+    constexpr int kRowsOf = kTcRows / (kSoftThreads / 32), kPer = D / 128;
+    float4 x[kRowsOf][kPer];
+#pragma unroll
+    for (int u = 0; u < kRowsOf; ++u) {
+      const int r = warp * kRowsOf + u, i = (row0 + r) / p.group, g = (row0 + r) - i * p.group;
+      const float4* src = reinterpret_cast<const float4*>(p.t.q + (static_cast<size_t>(i) * p.t.heads + kv * p.group + g) * D) + lane;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) x[u][k] = r < rows ? __ldg(src + k * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
     if (row < rows) {
       int length = 0;
 #pragma unroll
       for (int w = 0; w < kTreeWords; ++w) length += __popc(sh.path[tree_i][w]);
-      seeing = length != 0;
-      if (seeing) first = p.t.window != 0 ? max(0, n - (p.t.window - length)) : 0;
+      if (length != 0) first = p.t.window != 0 ? max(0, n - (p.t.window - length)) : 0;
     }
-    const float4* src = reinterpret_cast<const float4*>(p.t.q + (static_cast<size_t>(tree_i) * p.t.heads + head) * D + half * (D / 2));
-    float4 x[D / 8];
-    float most = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) x[i] = seeing ? __ldg(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const float a = fmaxf(fabsf(x[i].x), fabsf(x[i].y)), b = fmaxf(fabsf(x[i].z), fabsf(x[i].w));
-      most = fmaxf(most, fmaxf(a, b));
-    }
-    sh.q_most[half][row] = most;
+    if (half == 0) sh.first[row] = first;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    most = fmaxf(most, sh.q_most[half ^ 1][row]);
-    int e = static_cast<int>((__float_as_uint(most) >> 23) & 0xFFu) - 127 - 13;
-    e = most == 0.0f ? 0 : max(-110, min(114, e));
-    const float up = power_of_two(-e);
-    row_f = power_of_two(e) * (kLog2e / sqrtf(static_cast<float>(D)));
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      uint32_t hi[16], lo[16];
+    for (int u = 0; u < kRowsOf; ++u) {
+      const int r = warp * kRowsOf + u;
+      const bool used = sh.first[r] != kUnused;
+      uint32_t most = 0;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float4 y = x[i * 8 + u];
-        tree_split(y.x * up, y.y * up, hi[2 * u], lo[2 * u]);
-        tree_split(y.z * up, y.w * up, hi[2 * u + 1], lo[2 * u + 1]);
+      for (int k = 0; k < kPer; ++k) {
+        if (!used) x[u][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        most = max(max(most, max(__float_as_uint(x[u][k].x) & 0x7FFFFFFFu, __float_as_uint(x[u][k].y) & 0x7FFFFFFFu)),
+                   max(__float_as_uint(x[u][k].z) & 0x7FFFFFFFu, __float_as_uint(x[u][k].w) & 0x7FFFFFFFu));
       }
-      tc_store16(tmem + lanes + kColQ + half * (D / 4) + i * 16, hi);
-      tc_store16(tmem + lanes + kColQ + D / 2 + half * (D / 4) + i * 16, lo);
+      most = __reduce_max_sync(0xFFFFFFFFu, most);
+      const int e = most == 0 ? 0 : max(-110, min(114, static_cast<int>(most >> 23) - 127 - 13));
+      const float up = power_of_two(-e);
+      if (lane == 0) sh.q_unit[r] = power_of_two(e);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) x[u][k] = make_float4(x[u][k].x * up, x[u][k].y * up, x[u][k].z * up, x[u][k].w * up);
     }
-    tc_store_wait();
+    constexpr int kHalfPieces = D / 8;  // 16-byte pieces of half a row
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int u = 0; u < kRowsOf; ++u) {
+        const int r = warp * kRowsOf + u;
+        if (kPer == 2 || lane / kHalfPieces == h)
+          *reinterpret_cast<float4*>(v_s + r * (D * 2) + (((lane % kHalfPieces) ^ (r & 7)) << 4)) = x[u][kPer == 2 ? h : 0];
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (half == h) {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float4 y = *reinterpret_cast<const float4*>(v_s + row * (D * 2) + (((i * 8 + u) ^ (row & 7)) << 4));
+            tree_split(y.x, y.y, hi[2 * u], lo[2 * u]);
+            tree_split(y.z, y.w, hi[2 * u + 1], lo[2 * u + 1]);
+          }
+          tc_store16(tmem + lanes + kColQ + half * (D / 4) + i * 16, hi);
+          tc_store16(tmem + lanes + kColQ + D / 2 + half * (D / 4) + i * 16, lo);
+        }
+        tc_store_wait();
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    row_f = sh.q_unit[row] * (kLog2e / sqrtf(static_cast<float>(D)));
   }
   tc_before();
   __syncthreads();
   tc_after();
+  if (KV == kKvF16 && loading) loader.fetch(true, 0, v_s, load_tid), loader.fetch(true, 1, v_s + S::kTileBytes, load_tid);
 
   // the softmax warps hold 128 sums a thread where head_dim is 256: 256 * 208 + 128 * 88 registers, the launch's 384 * 168
   if (D == 256) {
@@ -626,19 +655,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       if (lane == 0) mbar_arrive(&sh.o_read);
     };
     for (int t = 0; t < tiles; ++t) {
-      wait(&sh.s_full, t);
+      const uint32_t s_at = tmem + lanes + kColS + (t & 1) * 64;
+      wait(&sh.s_full[t & 1], t >> 1);
       tc_after();
       uint32_t s[32];
-      tc_load32(tmem + lanes + kColS + half * 32, s);
-      tc_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.s_read);
+      tc_load32(s_at + half * 32, s);
       if (KV == kKvF32) wait(&sh.v_full[t % S::kVBufs], t / S::kVBufs);  // (their scales come with the values)
       // which of the 32 keys the row sees
       const int j0 = c0 + t * kTcKeys + half * 32;
       uint32_t see = 0xFFFFFFFFu;
       if (j0 < first || j0 + 32 > n) {
-        see = first == 0x7FFFFFFF ? 0u : bits_between(first - j0, n - j0);
+        see = first == kUnused ? 0u : bits_between(first - j0, n - j0);
         const int off = j0 - n;
         if (off > -32 && row < rows) {
           const uint32_t* path = sh.path[tree_i];
@@ -663,9 +690,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
         for (int c = 0; c < 32; ++c)
           if (!(see >> c & 1u)) s[c] = 0xFF800000u;
       }
-      float top = -INFINITY;
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(s[c]));
+      for (int c = 0; c < 32; ++c) tops[c & 3] = fmaxf(tops[c & 3], __uint_as_float(s[c]));
+      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       sh.top[t & 1][half][row] = top;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       top = fmaxf(top, sh.top[t & 1][half ^ 1][row]);
@@ -717,18 +745,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       }
       const float next_unit = power_of_two(e - 14);
       sum = fmaf(part[0] + part[1], next_unit, sum * corr);
-      // the tile before: its second half (its only one where head_dim is 128) leaves the weights' columns free
-      if (t > 0) {
-        wait(&sh.o_full, S::kHalves * t - 1);
-        tc_after();
-        take(o[S::kHalves - 1]);
-      }
-      tc_store16(tmem + lanes + kColP + half * 16, hi);
-      tc_store16(tmem + lanes + kColP + 32 + half * 16, lo);
+      // the weights over the scores (the other half's threads have read theirs: they were at the barrier above)
+      tc_store16(s_at + half * 16, hi);
+      tc_store16(s_at + 32 + half * 16, lo);
       tc_store_wait();
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full);
+      if (lane == 0) mbar_arrive(&sh.p_full[t & 1]);
+      // the outputs of the tile before
+      if (t > 0) {
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h) {
+          wait(&sh.o_full, S::kHalves * (t - 1) + h);
+          tc_after();
+          take(o[h]);
+        }
+      }
       if (__any_sync(0xFFFFFFFFu, corr != 1.0f)) {
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h)
@@ -736,15 +768,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
           for (int c = 0; c < 64; ++c) o[h][c] *= corr;
       }
       unit = next_unit;
-      if (S::kHalves == 2) {
-        wait(&sh.o_full, 2 * t);
-        tc_after();
-        take(o[0]);
-      }
     }
-    wait(&sh.o_full, S::kHalves * tiles - 1);
-    tc_after();
-    take(o[S::kHalves - 1]);
+#pragma unroll
+    for (int h = 0; h < S::kHalves; ++h) {
+      wait(&sh.o_full, S::kHalves * (tiles - 1) + h);
+      tc_after();
+      take(o[h]);
+    }
     // A NaN or an infinity among a row's operands has made its sums so (that of a key which it does not see as well: its
     // weight of 0 does not mask it).
     float all = sum;
@@ -756,17 +786,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     if (!(fabsf(all) <= 3.402823466e38f)) sh.bad[row] = sh.any_bad = 1;
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (sh.any_bad != 0) tree_scalar_rows<KV, D>(p, sh, kv, row0, rows, c0, c1, split);
-    if (row < rows && sh.bad[row] == 0) {
-      sum += sh.sum[half ^ 1][row];
-      const size_t at = static_cast<size_t>(tree_i) * p.t.heads + head;
-      float* dst = p.pacc != nullptr ? p.pacc + (at * p.splits + split) * D : p.t.out + at * D;
-      const float f = p.pacc != nullptr ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    // through shared memory, so that a warp writes whole rows; the operands' buffers are free
+    sum += sh.sum[half ^ 1][row];
+    const float f = p.pacc != nullptr ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-      for (int h = 0; h < S::kHalves; ++h)
+    for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-        for (int c = 0; c < 64; c += 4)
-          *reinterpret_cast<float4*>(dst + h * 128 + half * 64 + c) = make_float4(o[h][c] * f, o[h][c + 1] * f, o[h][c + 2] * f, o[h][c + 3] * f);
-      if (p.pacc != nullptr && half == 0) p.pmax[at * p.splits + split] = mx, p.psum[at * p.splits + split] = sum;
+      for (int c = 0; c < 64; c += 4)
+        *reinterpret_cast<float4*>(smem + row * (D * 4) + (((h * 32 + half * 16 + c / 4) ^ (row & 7)) << 4)) =
+            make_float4(o[h][c] * f, o[h][c + 1] * f, o[h][c + 2] * f, o[h][c + 3] * f);
+    if (half == 0) sh.top[0][0][row] = mx, sh.top[0][1][row] = sum;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    for (int r = warp; r < rows; r += kSoftThreads / 32) {
+      if (sh.bad[r] != 0) continue;
+      const int i = (row0 + r) / p.group;
+      const size_t at = static_cast<size_t>(i) * p.t.heads + kv * p.group + (row0 + r) - i * p.group;
+      float4* dst = reinterpret_cast<float4*>(p.pacc != nullptr ? p.pacc + (at * p.splits + split) * D : p.t.out + at * D);
+#pragma unroll
+      for (int k = 0; k < D / 128; ++k) dst[k * 32 + lane] = *reinterpret_cast<const float4*>(smem + r * (D * 4) + (((k * 32 + lane) ^ (r & 7)) << 4));
+      if (p.pacc != nullptr && lane == 0) p.pmax[at * p.splits + split] = sh.top[0][0][r], p.psum[at * p.splits + split] = sh.top[0][1][r];
     }
   } else if (loading) {
     float k_next = 0.0f, v_next = 0.0f;  // the next tile's scales
@@ -822,54 +860,58 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
   } else if (lane == 0) {
     const uint32_t s_shape = tc_shape(kTcKeys, false), o_shape = tc_shape(128, true);
     auto scores = [&](int t) {
+      const uint32_t d = tmem + kColS + (t & 1) * 64;
       const uint32_t at = smem_u32(k_s + (t % S::kKBufs) * S::kTileBytes);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {  // the small products first
         const uint64_t b = tc_operand(at + kk * 256, 128, S::kGroupBytes);
-        tc_mma(tmem + kColS, tmem + kColQ + D / 2 + kk * 8, b, s_shape, kk != 0);
-        if (S::kTerms == 2) tc_mma(tmem + kColS, tmem + kColQ + kk * 8, tc_operand(at + S::kTermBytes + kk * 256, 128, S::kGroupBytes), s_shape, 1);
+        tc_mma(d, tmem + kColQ + D / 2 + kk * 8, b, s_shape, kk != 0);
+        if (S::kTerms == 2) tc_mma(d, tmem + kColQ + kk * 8, tc_operand(at + S::kTermBytes + kk * 256, 128, S::kGroupBytes), s_shape, 1);
       }
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
-        tc_mma(tmem + kColS, tmem + kColQ + kk * 8, tc_operand(at + kk * 256, 128, S::kGroupBytes), s_shape, 1);
-      tc_commit(&sh.s_full);
+        tc_mma(d, tmem + kColQ + kk * 8, tc_operand(at + kk * 256, 128, S::kGroupBytes), s_shape, 1);
+      tc_commit(&sh.s_full[t & 1]);
       tc_commit(&sh.k_empty[t % S::kKBufs]);
     };
     auto outputs = [&](int t, int h) {
+      const uint32_t w = tmem + kColS + (t & 1) * 64;
       const uint32_t at = smem_u32(v_s + (t % S::kVBufs) * S::kTileBytes) + h * 2048;
 #pragma unroll
       for (int kk = 0; kk < kTcKeys / 16; ++kk) {
         const uint64_t b = tc_operand(at + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128);
-        tc_mma(tmem + kColO, tmem + kColP + 32 + kk * 8, b, o_shape, kk != 0);
-        if (S::kTerms == 2) tc_mma(tmem + kColO, tmem + kColP + kk * 8, tc_operand(at + S::kTermBytes + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128), o_shape, 1);
+        tc_mma(tmem + kColO, w + 32 + kk * 8, b, o_shape, kk != 0);
+        if (S::kTerms == 2) tc_mma(tmem + kColO, w + kk * 8, tc_operand(at + S::kTermBytes + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128), o_shape, 1);
       }
 #pragma unroll
       for (int kk = 0; kk < kTcKeys / 16; ++kk)
-        tc_mma(tmem + kColO, tmem + kColP + kk * 8, tc_operand(at + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128), o_shape, 1);
+        tc_mma(tmem + kColO, w + kk * 8, tc_operand(at + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128), o_shape, 1);
       tc_commit(&sh.o_full);
       if (h == S::kHalves - 1) tc_commit(&sh.v_empty[t % S::kVBufs]);
     };
-    wait(&sh.k_full[0], 0);
-    tc_after();
-    if (ok) scores(0);
+    auto next_scores = [&](int t) {
+      if (t >= tiles) return;
+      wait(&sh.k_full[t % S::kKBufs], t / S::kKBufs);
+      tc_after();
+      if (ok) scores(t);
+    };
+    next_scores(0);
+    next_scores(1);
     for (int t = 0; t < tiles && ok; ++t) {
       // outputs of a half: the weights and values are there, and the half before has been read
-      wait(&sh.p_full, t);
+      wait(&sh.p_full[t & 1], t >> 1);
       wait(&sh.v_full[t % S::kVBufs], t / S::kVBufs);
-      if (t > 0) wait(&sh.o_read, S::kHalves * t - 1);
-      tc_after();
-      if (ok) outputs(t, 0);
-      if (t + 1 < tiles) {
-        wait(&sh.s_read, t);
-        wait(&sh.k_full[(t + 1) % S::kKBufs], (t + 1) / S::kKBufs);
+#pragma unroll
+      for (int h = 0; h < S::kHalves; ++h) {
+        if (t + h > 0) wait(&sh.o_read, S::kHalves * t + h - 1);
         tc_after();
-        if (ok) scores(t + 1);
+        if (ok) outputs(t, h);
       }
-      if (S::kHalves == 2) {
-        wait(&sh.o_read, 2 * t);
-        tc_after();
-        if (ok) outputs(t, 1);
-      }
+      next_scores(t + 2);  // over this tile's weights, behind the products that read them
+    }
+    if (!ok) {  // products may be under way still: not while tensor memory is given back
+      tc_commit(&sh.drained);
+      mbar_wait(&sh.drained, 0, &g_tree_timeouts);
     }
   }
   __syncwarp();
