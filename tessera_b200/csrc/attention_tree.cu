@@ -148,21 +148,24 @@ struct TcParams {
 template <int KV, int D>
 struct TcShape {
   static constexpr int kTerms = KV == kKvF32 ? 2 : 1;
-  static constexpr int kKBufs = KV == kKvF32 ? 1 : 2, kVBufs = 2;  // of a tile's keys and of its values
+  static constexpr int kBufs = KV == kKvF32 ? 1 : 2;  // of a tile's keys and of its values
   static constexpr int kTermBytes = kTcKeys * D * 2, kTileBytes = kTerms * kTermBytes;
   static constexpr int kRowBytes = D * kv_bits<KV>() / 8;
   static constexpr bool kRaw = KV != kKvF32 && KV != kKvF16;          // raw bytes pass through shared memory
+  static constexpr int kBox = kRowBytes < 128 ? kRowBytes : 128;      // bytes of a key in a box of raw bytes; 128: swizzled
   static constexpr int kRawBytes = kRaw ? kTcKeys * kRowBytes : 0;
+  static constexpr int kRun = 4, kRuns = 5, kRunsOfTile = (kTcKeys / (kLoadThreads / 32) + kRun) / kRun;  // fp32: rows of a warp under way
+  static constexpr int kRing = KV == kKvF32 ? kLoadThreads / 32 * kRuns * kRun * kRowBytes : 0;
   static constexpr int kHalves = D / 128;
   static constexpr uint32_t kGroupBytes = D / 8 * 128;                // eight keys
-  static constexpr int kSmem = 1024 + (kKBufs + kVBufs) * kTileBytes + 4 * kRawBytes;
+  static constexpr int kSmem = 1024 + 2 * kBufs * kTileBytes + 4 * kRawBytes + kRing;
 };
 
 // A parity wait tells a phase from the one before it, so no barrier may come two phases ahead of one who waits on it: scores and
 // weights have a barrier for either buffer, since the softmax warps give away a tile's weights before the MMAs have taken the
 // tile's before it; a phase of each other one is followed by the next only when everybody who waits for it has been heard of.
 struct TcShared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_read, drained;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_read, drained, raw_full[2][2];
   uint32_t tmem;
   uint32_t used[kTreeWords];               // rows of the tree that are used
   uint32_t path[kTreeRows][kTreeWords + 1];  // what each row sees of the tree
@@ -171,10 +174,8 @@ struct TcShared {
   int range[kScaleBufs][kLoadThreads / 32][2];      // largest and smallest exponent of the values' scales
   float top[2][2][kTcRows];                         // [tile & 1][half of the keys][row]: largest score
   float weighed[2][kTcRows];                        // the same of score + log2 of the value's scale
-  int first[kTcRows];                               // the first past row that a row sees (kUnused: it is not used)
-  float q_unit[kTcRows];
+  uint32_t q_most[2][kTcRows];
   float sum[2][kTcRows];
-  int bad[kTcRows], any_bad;                        // rows with something that is not finite
 };
 
 __device__ __forceinline__ void tc_alloc(uint32_t* slot) {
@@ -332,44 +333,41 @@ __device__ __forceinline__ void tree_paths(TcShared& sh, int m, int window) {
   __syncthreads();
 }
 
-// The marked rows of the CTA over keys [c0, c1), a warp a row and key by key in fp32: where something is not finite.
+// Pair r of (tree row, head) over keys [c0, c1), by a warp and key by key in fp32: where something is not finite.
 template <int KV, int D>
-__device__ __noinline__ void tree_scalar_rows(const TcParams& p, const TcShared& sh, int kv, int row0, int rows, int c0, int c1, int split) {
+__device__ __noinline__ void tree_scalar_row(const TcParams& p, const TcShared& sh, int kv, int r, int c0, int c1, int split) {
   constexpr bool kScaled = KV >= kKvFp8;
   constexpr size_t kRowBytes = static_cast<size_t>(D) * kv_bits<KV>() / 8;
   const int lane = threadIdx.x & 31, n = p.t.n;
   const size_t row_bytes = p.t.kv_heads * kRowBytes;
-  for (int r = threadIdx.x >> 5; r < rows; r += kSoftThreads / 32) {
-    if (sh.bad[r] == 0) continue;
-    const int i = (row0 + r) / p.group, h = kv * p.group + (row0 + r) - i * p.group;
-    int length = 0;
-    for (int w = 0; w < kTreeWords; ++w) length += __popc(sh.path[i][w]);
-    const int first = length == 0 ? n : p.t.window != 0 ? max(0, n - (p.t.window - length)) : 0;
-    const size_t at = (static_cast<size_t>(i) * p.t.heads + h) * D;
-    float x[D / 32], acc[D / 32], top = kNoKey, total = 0.0f;
+  const int i = r / p.group, h = kv * p.group + r - i * p.group;
+  int length = 0;
+  for (int w = 0; w < kTreeWords; ++w) length += __popc(sh.path[i][w]);
+  const int first = length == 0 ? n : p.t.window != 0 ? max(0, n - (p.t.window - length)) : 0;
+  const size_t at = (static_cast<size_t>(i) * p.t.heads + h) * D;
+  float x[D / 32], acc[D / 32], top = kNoKey, total = 0.0f;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) x[e] = p.t.q[at + e * 32 + lane] * (kLog2e / sqrtf(static_cast<float>(D))), acc[e] = 0.0f;
-    for (int j = max(first, c0); j < c1; ++j) {
-      if (j >= n && !(sh.path[i][(j - n) >> 5] >> ((j - n) & 31) & 1u)) continue;
-      const unsigned char *kr = p.t.k + j * row_bytes + kv * kRowBytes, *vr = p.t.v + j * row_bytes + kv * kRowBytes;
-      float dot = 0.0f;
+  for (int e = 0; e < D / 32; ++e) x[e] = p.t.q[at + e * 32 + lane] * (kLog2e / sqrtf(static_cast<float>(D))), acc[e] = 0.0f;
+  for (int j = max(first, c0); j < c1; ++j) {
+    if (j >= n && !(sh.path[i][(j - n) >> 5] >> ((j - n) & 31) & 1u)) continue;
+    const unsigned char *kr = p.t.k + j * row_bytes + kv * kRowBytes, *vr = p.t.v + j * row_bytes + kv * kRowBytes;
+    float dot = 0.0f;
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) dot = fmaf(x[e], tree_element<KV>(kr, e * 32 + lane), dot);
-      const float sc = warp_sum(dot) * (kScaled ? p.t.ks[j] : 1.0f), now = fmaxf(top, sc);
-      const float corr = exp2f(top - now), w = exp2f(sc - now), wv = w * (kScaled ? p.t.vs[j] : 1.0f);
-      total = fmaf(total, corr, w);
+    for (int e = 0; e < D / 32; ++e) dot = fmaf(x[e], tree_element<KV>(kr, e * 32 + lane), dot);
+    const float sc = warp_sum(dot) * (kScaled ? p.t.ks[j] : 1.0f), now = fmaxf(top, sc);
+    const float corr = exp2f(top - now), w = exp2f(sc - now), wv = w * (kScaled ? p.t.vs[j] : 1.0f);
+    total = fmaf(total, corr, w);
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wv, tree_element<KV>(vr, e * 32 + lane), acc[e] * corr);
-      top = now;
-    }
-    const size_t part = (static_cast<size_t>(i) * p.t.heads + h) * p.splits + split;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      if (p.pacc != nullptr) p.pacc[part * D + e * 32 + lane] = acc[e];
-      else p.t.out[at + e * 32 + lane] = total == 0.0f ? 0.0f : acc[e] / total;
-    }
-    if (p.pacc != nullptr && lane == 0) p.pmax[part] = top, p.psum[part] = total;
+    for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wv, tree_element<KV>(vr, e * 32 + lane), acc[e] * corr);
+    top = now;
   }
+  const size_t part = (static_cast<size_t>(i) * p.t.heads + h) * p.splits + split;
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) {
+    if (p.pacc != nullptr) p.pacc[part * D + e * 32 + lane] = acc[e];
+    else p.t.out[at + e * 32 + lane] = total == 0.0f ? 0.0f : acc[e] / total;
+  }
+  if (p.pacc != nullptr && lane == 0) p.pmax[part] = top, p.psum[part] = total;
 }
 
 // The loading warps' part: tile t of the keys (VALUES: of the values) into its operand buffer, raw bytes from `raw`.
@@ -378,6 +376,7 @@ struct TcLoader {
   using S = TcShape<KV, D>;
   const TcParams& p;
   TcShared& sh;
+  const CUtensorMap *k_map, *v_map;
   int kv, c0, c1, tiles;
 
   __device__ __forceinline__ const unsigned char* base(bool values) const {
@@ -395,18 +394,26 @@ struct TcLoader {
   static __device__ __forceinline__ int key_of(int it, int lane) { return (it & 7) * 8 + (lane & 7); }
   static __device__ __forceinline__ int piece_of(int it, int lane) { return (it >> 3) * 4 + (lane >> 3); }
   static __device__ __forceinline__ uint32_t operand_at(int it, int lane, int c) { return (it & 7) * S::kGroupBytes + (lane & 7) * 16 + c * 128; }
-  __device__ __forceinline__ void fetch(bool values, int t, unsigned char* dst, int tid) const {  // raw bytes, or fp16 in place
+  // Raw bytes, by one thread (rows beyond the cache's last come as zeros).
+  __device__ __forceinline__ void fetch_raw(bool values, int t, unsigned char* raw) const {
+    if (t >= tiles) return;
+    uint64_t* bar = &sh.raw_full[t & 1][values ? 1 : 0];
+    mbar_expect_tx(bar, S::kRawBytes);
+#pragma unroll
+    for (int b = 0; b < S::kRowBytes / S::kBox; ++b)
+      tma_load_2d(raw + b * kTcKeys * S::kBox, values ? v_map : k_map, kv * S::kRowBytes + b * S::kBox, c0 + t * kTcKeys, bar);
+  }
+  // fp16: straight into the operand's layout
+  __device__ __forceinline__ void fetch(bool values, int t, unsigned char* dst, int tid) const {
     if (t < tiles) {
       const int warp = tid >> 5, lane = tid & 31, j0 = c0 + t * kTcKeys;
       const unsigned char* src = base(values) + static_cast<size_t>(j0) * pitch();
       const int last = c1 - 1 - j0;
-      const uint32_t step = static_cast<uint32_t>(pitch());
 #pragma unroll 4
       for (int it = warp; it < kTimes; it += kLoadThreads / 32) {
         const int c = piece_of(it, lane);
-        const uint32_t at = KV == kKvF16 ? operand_at(it, lane, c) : it * 512 + lane * 16;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + at),
-                     "l"(src + static_cast<size_t>(min(key_of(it, lane), last)) * step + c * 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + operand_at(it, lane, c)),
+                     "l"(src + static_cast<size_t>(min(key_of(it, lane), last)) * pitch() + c * 16)
                      : "memory");
       }
     }
@@ -416,53 +423,94 @@ struct TcLoader {
   __device__ __forceinline__ void convert(int t, const unsigned char* raw, unsigned char* dst, int tid) const {
     const int warp = tid >> 5, lane = tid & 31, j0 = c0 + t * kTcKeys;
     const bool past = j0 + kTcKeys <= p.t.n;
-    if (KV == kKvF16 && past) return;
-#pragma unroll 4
-    for (int it = warp; it < kTimes; it += kLoadThreads / 32) {
-      const int c = piece_of(it, lane);
-      const bool zero = !past && unseen(min(j0 + key_of(it, lane), c1 - 1));
-      if constexpr (KV == kKvF16) {
-        if (zero) *reinterpret_cast<uint4*>(dst + operand_at(it, lane, c)) = make_uint4(0u, 0u, 0u, 0u);
-      } else {
-        constexpr int kWords = KV == kKvInt4 ? 4 : 2;  // of 16 bytes of operand a piece becomes
-        uint4 y = *reinterpret_cast<const uint4*>(raw + it * 512 + lane * 16);
-        if (zero) y = make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-        uint32_t h[4][KV == kKvInt4 ? 4 : 2];
+    if constexpr (KV == kKvF16) {
+      if (past) return;
+      for (int it = warp; it < kTimes; it += kLoadThreads / 32)
+        if (unseen(min(j0 + key_of(it, lane), c1 - 1)))
+          *reinterpret_cast<uint4*>(dst + operand_at(it, lane, piece_of(it, lane))) = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      constexpr int kWords = KV == kKvInt4 ? 4 : 2;  // of 16 bytes of operand a piece becomes
+      constexpr int kRun = KV == kKvInt4 ? 2 : 4;    // pieces in flight
+      auto raw_at = [&](int it) {  // piece c of a key lies at c ^ (key & 7) of its 128 bytes
+        const int c = piece_of(it, lane), key = key_of(it, lane);
+        return S::kBox == 128 ? raw + (c >> 3) * (kTcKeys * 128) + key * 128 + (((c ^ key) & 7) << 4) : raw + key * S::kBox + c * 16;
+      };
+#pragma unroll 1
+      for (int i0 = warp; i0 < kTimes; i0 += kRun * (kLoadThreads / 32)) {
+        uint4 y[kRun];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tree_expand<KV>(w[i], h[i]);
+        for (int u = 0; u < kRun; ++u) {
+          const int it = min(i0 + u * (kLoadThreads / 32), kTimes - 1);
+          y[u] = *reinterpret_cast<const uint4*>(raw_at(it));
+          if (!past && unseen(min(j0 + key_of(it, lane), c1 - 1))) y[u] = make_uint4(0u, 0u, 0u, 0u);
+        }
 #pragma unroll
-        for (int o = 0; o < kWords; ++o) {
-          const uint4 z = KV == kKvInt4 ? make_uint4(h[o][0], h[o][1], h[o][2 % kWords], h[o][3 % kWords])
-                                        : make_uint4(h[2 * (o & 1)][0], h[2 * (o & 1)][1], h[2 * (o & 1) + 1][0], h[2 * (o & 1) + 1][1]);
-          *reinterpret_cast<uint4*>(dst + operand_at(it, lane, c * kWords + o)) = z;
+        for (int u = 0; u < kRun; ++u) {
+          const int it = i0 + u * (kLoadThreads / 32);
+          const uint32_t w[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+          uint32_t h[4][KV == kKvInt4 ? 4 : 2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tree_expand<KV>(w[i], h[i]);
+          unsigned char* at = dst + operand_at(it, lane, piece_of(it, lane) * kWords);
+          if (it < kTimes) {
+#pragma unroll
+            for (int o = 0; o < kWords; ++o)
+              *reinterpret_cast<uint4*>(at + o * 128) = KV == kKvInt4 ? make_uint4(h[o][0], h[o][1], h[o][2 % kWords], h[o][3 % kWords])
+                                                                     : make_uint4(h[2 * (o & 1)][0], h[2 * (o & 1)][1], h[2 * (o & 1) + 1][0], h[2 * (o & 1) + 1][1]);
+          }
         }
       }
     }
   }
-  // fp32 rows, a warp each: scaled by a power of two to [2^13, 2^14), two terms
-  __device__ __forceinline__ void split_rows(bool values, int t, unsigned char* dst, int tid) const {
-    constexpr int kLoadWarps = kLoadThreads / 32, kRun = 512 / D, kPer = D / 128;
+  // fp32 rows pass through a warp's own ring, a run of four at a time and four runs ahead; a lane reads what it asked for.
+  // Run s of a warp: tile s / (2 kRunsOfTile), its keys first, then its values.
+  __device__ __forceinline__ void ask_rows(int s, unsigned char* ring, int tid) const {
+    const int lane = tid & 31, warp = tid >> 5;
+    if (s < tiles * 2 * S::kRunsOfTile) {
+      const int t = s / (2 * S::kRunsOfTile), x = s - t * 2 * S::kRunsOfTile;
+      const bool values = x >= S::kRunsOfTile;
+      const int k0 = (values ? x - S::kRunsOfTile : x) * S::kRun * (kLoadThreads / 32) + warp;
+      unsigned char* dst = ring + ((warp * S::kRuns + s % S::kRuns) * S::kRun) * S::kRowBytes + lane * 16;
+#pragma unroll
+      for (int u = 0; u < S::kRun; ++u) {
+        const int key = k0 + u * (kLoadThreads / 32), j = min(c0 + t * kTcKeys + key, c1 - 1);
+        const unsigned char* src = base(values) + j * pitch() + lane * 16;
+        if (key < kTcKeys) {
+#pragma unroll
+          for (int i = 0; i < D / 128; ++i)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + u * S::kRowBytes + i * 512), "l"(src + i * 512) : "memory");
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // Each row scaled by a power of two to [2^13, 2^14), two terms.
+  __device__ __forceinline__ void split_rows(bool values, int t, unsigned char* ring, unsigned char* dst, int tid) const {
+    constexpr int kLoadWarps = kLoadThreads / 32, kPer = D / 128;
     const int lane = tid & 31, warp = tid >> 5;
     int high = kNoExponent, low = -kNoExponent;
-    for (int k0 = warp; k0 < kTcKeys; k0 += kLoadWarps * kRun) {
-      float4 x[kRun][kPer];
+#pragma unroll 1
+    for (int b = 0; b < S::kRunsOfTile; ++b) {
+      const int s = (2 * t + (values ? 1 : 0)) * S::kRunsOfTile + b;
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kRuns - 1) : "memory");
+      const unsigned char* src = ring + ((warp * S::kRuns + s % S::kRuns) * S::kRun) * S::kRowBytes + lane * 16;
+      float4 x[S::kRun][kPer];
 #pragma unroll
-      for (int u = 0; u < kRun; ++u) {
-        const int key = k0 + u * kLoadWarps, j = min(c0 + t * kTcKeys + key, c1 - 1);
-        const float4* src = reinterpret_cast<const float4*>(base(values) + j * pitch()) + lane;
+      for (int u = 0; u < S::kRun; ++u)
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[u][i] = key < kTcKeys && !unseen(j) ? __ldg(src + i * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+        for (int i = 0; i < kPer; ++i) x[u][i] = *reinterpret_cast<const float4*>(src + u * S::kRowBytes + i * 512);
 #pragma unroll
-      for (int u = 0; u < kRun; ++u) {
-        const int key = k0 + u * kLoadWarps;
+      for (int u = 0; u < S::kRun; ++u) {
+        const int key = (b * S::kRun + u) * kLoadWarps + warp;
         if (key >= kTcKeys) break;
         uint32_t most = 0;
+        const bool zero = unseen(min(c0 + t * kTcKeys + key, c1 - 1));
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
+        for (int i = 0; i < kPer; ++i) {
+          if (zero) x[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
           most = max(max(most, max(__float_as_uint(x[u][i].x) & 0x7FFFFFFFu, __float_as_uint(x[u][i].y) & 0x7FFFFFFFu)),
                      max(__float_as_uint(x[u][i].z) & 0x7FFFFFFFu, __float_as_uint(x[u][i].w) & 0x7FFFFFFFu));
+        }
         most = __reduce_max_sync(0xFFFFFFFFu, most);
         const int e = most == 0 ? 0 : max(-110, min(114, static_cast<int>(most >> 23) - 127 - 13));
         const float up = power_of_two(-e);
@@ -479,6 +527,7 @@ struct TcLoader {
           *reinterpret_cast<uint2*>(at + S::kTermBytes) = lo;
         }
       }
+      ask_rows(s + S::kRuns, ring, tid);
     }
     if (values && lane == 0) sh.range[t % kScaleBufs][warp][0] = high, sh.range[t % kScaleBufs][warp][1] = low;
   }
@@ -499,15 +548,16 @@ struct TcLoader {
 };
 
 template <int KV, int D>
-__global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const TcParams p) {
+__global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                                         const TcParams p) {
   using S = TcShape<KV, D>;
   constexpr bool kScaled = KV != kKvF16;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(16) TcShared sh;
   unsigned char* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char* const k_s = smem;                               // [kKBufs][terms][64 keys][D]
-  unsigned char* const v_s = k_s + S::kKBufs * S::kTileBytes;  // [kVBufs] ...
-  unsigned char* const raw_s = v_s + S::kVBufs * S::kTileBytes;  // [2][keys, values]
+  unsigned char* const k_s = smem;                               // [kBufs][terms][64 keys][D]
+  unsigned char* const v_s = k_s + S::kBufs * S::kTileBytes;
+  unsigned char* const raw_s = v_s + S::kBufs * S::kTileBytes;  // [2][keys, values]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kv = blockIdx.x % p.t.kv_heads, row0 = static_cast<int>(blockIdx.x) / p.t.kv_heads * kTcRows, split = blockIdx.y;
   const int rows = min(kTcRows, p.t.m * p.group - row0), n = p.t.n;
@@ -516,33 +566,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
   const int tiles = (c1 - c0 + kTcKeys - 1) / kTcKeys;
   const bool loading = warp >= kSoftThreads / 32 && warp < (kSoftThreads + kLoadThreads) / 32;
   const int load_tid = tid - kSoftThreads;
-  TcLoader<KV, D> loader{p, sh, kv, c0, c1, tiles};
+  TcLoader<KV, D> loader{p, sh, &k_map, &v_map, kv, c0, c1, tiles};
 
-  if (loading) {  // the first tiles are under way before anything else
-    if (S::kRaw) {
-      loader.fetch(false, 0, raw_s, load_tid), loader.fetch(true, 0, raw_s + S::kRawBytes, load_tid);
-      loader.fetch(false, 1, raw_s + 2 * S::kRawBytes, load_tid), loader.fetch(true, 1, raw_s + 3 * S::kRawBytes, load_tid);
-    } else if (KV == kKvF16) {  // (the queries pass through the values' buffers first)
-      loader.fetch(false, 0, k_s, load_tid), loader.fetch(false, 1, k_s + S::kTileBytes, load_tid);
-    }
-  }
   if (tid < kTreeWords) sh.used[tid] = 0;
-  if (tid < kTcRows) sh.bad[tid] = 0;
   if (tid < p.t.m) sh.parents[tid] = p.t.parents[tid];
   if (tid == 0) {
-    sh.any_bad = 0;
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.k_full[b], kLoadThreads / 32), mbar_init(&sh.v_full[b], kLoadThreads / 32);
       mbar_init(&sh.k_empty[b], 1), mbar_init(&sh.v_empty[b], 1);
     }
     mbar_init(&sh.s_full[0], 1), mbar_init(&sh.s_full[1], 1), mbar_init(&sh.o_full, 1), mbar_init(&sh.drained, 1);
+    for (int b = 0; b < 4; ++b) mbar_init(&sh.raw_full[b >> 1][b & 1], 1);
     mbar_init(&sh.p_full[0], kSoftThreads / 32), mbar_init(&sh.p_full[1], kSoftThreads / 32), mbar_init(&sh.o_read, kSoftThreads / 32);
     mbar_fence_init();
   }
   if (warp == kTcThreads / 32 - 1) tc_alloc(&sh.tmem);
+  // Queries, to begin with as they are, in the operands' buffers: 16-byte piece c of a row at c ^ (row & 7).
+  if (warp < kSoftThreads / 32) {
+    constexpr int kRowsOf = kTcRows / (kSoftThreads / 32);
+    const int r0 = warp * kRowsOf;
+    int i = (row0 + r0) / p.group, g = (row0 + r0) - i * p.group;
+#pragma unroll 4
+    for (int u = 0; u < kRowsOf; ++u) {
+      const int r = r0 + u;
+      const float* src = p.t.q + (static_cast<size_t>(i) * p.t.heads + kv * p.group + g) * D + lane * 4;
+      if (r < rows) {
+#pragma unroll
+        for (int k = 0; k < D / 128; ++k)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem) + r * (D * 4) + (((k * 32 + lane) ^ (r & 7)) << 4)), "l"(src + k * 128) : "memory");
+      }
+      if (++g == p.group) g = 0, ++i;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
   tc_before();
   __syncthreads();
   tc_after();
+  if (S::kRaw && load_tid == 0)  // raw bytes of the first tiles
+    for (int t = 0; t < 4; ++t) loader.fetch_raw((t & 1) != 0, t >> 1, raw_s + t * S::kRawBytes);
+  if (KV == kKvF32 && loading)
+    for (int s = 0; s < S::kRuns; ++s) loader.ask_rows(s, raw_s, load_tid);
   tree_paths(sh, p.t.m, p.t.window);
   const uint32_t tmem = sh.tmem;
   // a thread's row
@@ -552,76 +615,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
   float row_f = 0.0f;
   int first = kUnused;
   if (warp < kSoftThreads / 32) {
-    // Queries: a warp reads its sixteen rows whole, scales each by a power of two to [2^13, 2^14) and leaves it in shared memory
-    // (16-byte piece c of a row at c ^ (row & 7)) half a row after the other; a thread takes half a row of two terms to tensor memory.
-    constexpr int kRowsOf = kTcRows / (kSoftThreads / 32), kPer = D / 128;
-    float4 x[kRowsOf][kPer];
-#pragma unroll
-    for (int u = 0; u < kRowsOf; ++u) {
-      const int r = warp * kRowsOf + u, i = (row0 + r) / p.group, g = (row0 + r) - i * p.group;
-      const float4* src = reinterpret_cast<const float4*>(p.t.q + (static_cast<size_t>(i) * p.t.heads + kv * p.group + g) * D) + lane;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) x[u][k] = r < rows ? __ldg(src + k * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+    // a thread half a row: scaled by a power of two to [2^13, 2^14), two terms to tensor memory
     if (row < rows) {
       int length = 0;
 #pragma unroll
       for (int w = 0; w < kTreeWords; ++w) length += __popc(sh.path[tree_i][w]);
       if (length != 0) first = p.t.window != 0 ? max(0, n - (p.t.window - length)) : 0;
     }
-    if (half == 0) sh.first[row] = first;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     asm volatile("bar.sync 1, 256;" ::: "memory");
-#pragma unroll
-    for (int u = 0; u < kRowsOf; ++u) {
-      const int r = warp * kRowsOf + u;
-      const bool used = sh.first[r] != kUnused;
-      uint32_t most = 0;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        if (!used) x[u][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        most = max(max(most, max(__float_as_uint(x[u][k].x) & 0x7FFFFFFFu, __float_as_uint(x[u][k].y) & 0x7FFFFFFFu)),
-                   max(__float_as_uint(x[u][k].z) & 0x7FFFFFFFu, __float_as_uint(x[u][k].w) & 0x7FFFFFFFu));
-      }
-      most = __reduce_max_sync(0xFFFFFFFFu, most);
-      const int e = most == 0 ? 0 : max(-110, min(114, static_cast<int>(most >> 23) - 127 - 13));
-      const float up = power_of_two(-e);
-      if (lane == 0) sh.q_unit[r] = power_of_two(e);
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) x[u][k] = make_float4(x[u][k].x * up, x[u][k].y * up, x[u][k].z * up, x[u][k].w * up);
+    const unsigned char* src = smem + row * (D * 4);
+    const int c0q = half * (D / 8);
+    uint32_t most = 0;
+#pragma unroll 4
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 y = *reinterpret_cast<const uint4*>(src + (((c0q + c) ^ (row & 7)) << 4));
+      most = max(max(most, max(y.x & 0x7FFFFFFFu, y.y & 0x7FFFFFFFu)), max(y.z & 0x7FFFFFFFu, y.w & 0x7FFFFFFFu));
     }
-    constexpr int kHalfPieces = D / 8;  // 16-byte pieces of half a row
+    sh.q_most[half][row] = most;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    most = first == kUnused ? 0u : max(most, sh.q_most[half ^ 1][row]);
+    const int e = most == 0 ? 0 : max(-110, min(114, static_cast<int>(most >> 23) - 127 - 13));
+    const float up = power_of_two(-e);
+    row_f = power_of_two(e) * (kLog2e / sqrtf(static_cast<float>(D)));
+#pragma unroll 1
+    for (int i = 0; i < D / 64; ++i) {
+      uint32_t hi[16], lo[16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int u = 0; u < kRowsOf; ++u) {
-        const int r = warp * kRowsOf + u;
-        if (kPer == 2 || lane / kHalfPieces == h)
-          *reinterpret_cast<float4*>(v_s + r * (D * 2) + (((lane % kHalfPieces) ^ (r & 7)) << 4)) = x[u][kPer == 2 ? h : 0];
+      for (int u = 0; u < 8; ++u) {
+        const float4 y = *reinterpret_cast<const float4*>(src + (((c0q + i * 8 + u) ^ (row & 7)) << 4));
+        tree_split(y.x * up, y.y * up, hi[2 * u], lo[2 * u]);
+        tree_split(y.z * up, y.w * up, hi[2 * u + 1], lo[2 * u + 1]);
+        if (first == kUnused) hi[2 * u] = hi[2 * u + 1] = lo[2 * u] = lo[2 * u + 1] = 0;  // (what the buffer holds may be anything)
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (half == h) {
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const float4 y = *reinterpret_cast<const float4*>(v_s + row * (D * 2) + (((i * 8 + u) ^ (row & 7)) << 4));
-            tree_split(y.x, y.y, hi[2 * u], lo[2 * u]);
-            tree_split(y.z, y.w, hi[2 * u + 1], lo[2 * u + 1]);
-          }
-          tc_store16(tmem + lanes + kColQ + half * (D / 4) + i * 16, hi);
-          tc_store16(tmem + lanes + kColQ + D / 2 + half * (D / 4) + i * 16, lo);
-        }
-        tc_store_wait();
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      tc_store16(tmem + lanes + kColQ + half * (D / 4) + i * 16, hi);
+      tc_store16(tmem + lanes + kColQ + D / 2 + half * (D / 4) + i * 16, lo);
     }
-    row_f = sh.q_unit[row] * (kLog2e / sqrtf(static_cast<float>(D)));
+    tc_store_wait();
   }
   tc_before();
   __syncthreads();
   tc_after();
-  if (KV == kKvF16 && loading) loader.fetch(true, 0, v_s, load_tid), loader.fetch(true, 1, v_s + S::kTileBytes, load_tid);
+  if (KV == kKvF16 && loading) {
+    loader.fetch(false, 0, k_s, load_tid), loader.fetch(true, 0, v_s, load_tid);
+    loader.fetch(false, 1, k_s + S::kTileBytes, load_tid), loader.fetch(true, 1, v_s + S::kTileBytes, load_tid);
+  }
 
   // the softmax warps hold 128 sums a thread where head_dim is 256: 256 * 208 + 128 * 88 registers, the launch's 384 * 168
   if (D == 256) {
@@ -654,13 +692,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.o_read);
     };
+    auto take_tile = [&](int t) {
+#pragma unroll
+      for (int h = 0; h < S::kHalves; ++h) {
+        wait(&sh.o_full, S::kHalves * t + h);
+        tc_after();
+        take(o[h]);
+      }
+    };
     for (int t = 0; t < tiles; ++t) {
       const uint32_t s_at = tmem + lanes + kColS + (t & 1) * 64;
       wait(&sh.s_full[t & 1], t >> 1);
       tc_after();
       uint32_t s[32];
       tc_load32(s_at + half * 32, s);
-      if (KV == kKvF32) wait(&sh.v_full[t % S::kVBufs], t / S::kVBufs);  // (their scales come with the values)
+      if (S::kBufs == 1) {  // a tile's values, whose scales come with them, wait for the products of the tile before
+        if (t > 0) take_tile(t - 1);
+        wait(&sh.v_full[0], t);
+      }
       // which of the 32 keys the row sees
       const int j0 = c0 + t * kTcKeys + half * 32;
       uint32_t see = 0xFFFFFFFFu;
@@ -752,15 +801,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       tc_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.p_full[t & 1]);
-      // the outputs of the tile before
-      if (t > 0) {
-#pragma unroll
-        for (int h = 0; h < S::kHalves; ++h) {
-          wait(&sh.o_full, S::kHalves * (t - 1) + h);
-          tc_after();
-          take(o[h]);
-        }
-      }
+      if (S::kBufs == 2 && t > 0) take_tile(t - 1);
       if (__any_sync(0xFFFFFFFFu, corr != 1.0f)) {
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h)
@@ -769,80 +810,84 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       }
       unit = next_unit;
     }
-#pragma unroll
-    for (int h = 0; h < S::kHalves; ++h) {
-      wait(&sh.o_full, S::kHalves * (tiles - 1) + h);
-      tc_after();
-      take(o[h]);
-    }
-    // A NaN or an infinity among a row's operands has made its sums so (that of a key which it does not see as well: its
-    // weight of 0 does not mask it).
-    float all = sum;
-#pragma unroll
-    for (int h = 0; h < S::kHalves; ++h)
-#pragma unroll
-      for (int c = 0; c < 64; ++c) all = fmaf(o[h][c], 0.0f, all);
+    take_tile(tiles - 1);
+    // Through shared memory (the operands' buffers are free), so that a warp writes whole rows.
     sh.sum[half][row] = sum;
-    if (!(fabsf(all) <= 3.402823466e38f)) sh.bad[row] = sh.any_bad = 1;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (sh.any_bad != 0) tree_scalar_rows<KV, D>(p, sh, kv, row0, rows, c0, c1, split);
-    // through shared memory, so that a warp writes whole rows; the operands' buffers are free
-    sum += sh.sum[half ^ 1][row];
-    const float f = p.pacc != nullptr ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
       for (int c = 0; c < 64; c += 4)
         *reinterpret_cast<float4*>(smem + row * (D * 4) + (((h * 32 + half * 16 + c / 4) ^ (row & 7)) << 4)) =
-            make_float4(o[h][c] * f, o[h][c + 1] * f, o[h][c + 2] * f, o[h][c + 3] * f);
-    if (half == 0) sh.top[0][0][row] = mx, sh.top[0][1][row] = sum;
+            make_float4(o[h][c], o[h][c + 1], o[h][c + 2], o[h][c + 3]);
+    if (half == 0) sh.top[0][0][row] = mx;
     asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 1
     for (int r = warp; r < rows; r += kSoftThreads / 32) {
-      if (sh.bad[r] != 0) continue;
       const int i = (row0 + r) / p.group;
       const size_t at = static_cast<size_t>(i) * p.t.heads + kv * p.group + (row0 + r) - i * p.group;
+      const float total = sh.sum[0][r] + sh.sum[1][r], f = p.pacc != nullptr ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
       float4* dst = reinterpret_cast<float4*>(p.pacc != nullptr ? p.pacc + (at * p.splits + split) * D : p.t.out + at * D);
+      float all = total;
+      float4 y[D / 128];
 #pragma unroll
-      for (int k = 0; k < D / 128; ++k) dst[k * 32 + lane] = *reinterpret_cast<const float4*>(smem + r * (D * 4) + (((k * 32 + lane) ^ (r & 7)) << 4));
-      if (p.pacc != nullptr && lane == 0) p.pmax[at * p.splits + split] = sh.top[0][0][r], p.psum[at * p.splits + split] = sh.top[0][1][r];
+      for (int k = 0; k < D / 128; ++k) {
+        y[k] = *reinterpret_cast<const float4*>(smem + r * (D * 4) + (((k * 32 + lane) ^ (r & 7)) << 4));
+        all = fmaf((y[k].x + y[k].y) + (y[k].z + y[k].w), 0.0f, all);
+      }
+      // A NaN or an infinity among a row's operands has made its sums so (that of a key which it does not see as well: its weight
+      // of 0 does not mask it).
+      if (!__all_sync(0xFFFFFFFFu, fabsf(all) <= 3.402823466e38f)) {
+        tree_scalar_row<KV, D>(p, sh, kv, row0 + r, c0, c1, split);
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < D / 128; ++k) dst[k * 32 + lane] = make_float4(y[k].x * f, y[k].y * f, y[k].z * f, y[k].w * f);
+      if (p.pacc != nullptr && lane == 0) p.pmax[at * p.splits + split] = sh.top[0][0][r], p.psum[at * p.splits + split] = total;
     }
   } else if (loading) {
     float k_next = 0.0f, v_next = 0.0f;  // the next tile's scales
     if (S::kRaw) loader.next_scales(0, load_tid, k_next, v_next);
     for (int t = 0; t < tiles; ++t) {
-      const int kb = t % S::kKBufs, k_use = t / S::kKBufs, vb = t % S::kVBufs, v_use = t / S::kVBufs;
+      const int kb = t % S::kBufs, k_use = t / S::kBufs, vb = t % S::kBufs, v_use = t / S::kBufs;
       unsigned char *const k_dst = k_s + kb * S::kTileBytes, *const v_dst = v_s + vb * S::kTileBytes;
-      unsigned char* const raw = raw_s + (t & 1) * 2 * S::kRawBytes;  // a thread reads the pieces that it fetched
+      unsigned char* const raw = raw_s + (t & 1) * 2 * S::kRawBytes;
       // keys: the buffer is free once the scores that read it are there
       if (KV != kKvF16 && k_use > 0) wait(&sh.k_empty[kb], k_use - 1);
       if constexpr (KV == kKvF32) {
-        loader.split_rows(false, t, k_dst, load_tid);
+        loader.split_rows(false, t, raw_s, k_dst, load_tid);
       } else {
-        if constexpr (S::kRaw) asm volatile("cp.async.wait_group 3;" ::: "memory");
-        else asm volatile("cp.async.wait_group 2;" ::: "memory");
-        loader.convert(t, raw, k_dst, load_tid);
         if constexpr (S::kRaw) {
           loader.put_scales(t, load_tid, k_next, v_next);
           loader.next_scales(t + 1, load_tid, k_next, v_next);
-          loader.fetch(false, t + 2, raw, load_tid);
+          wait(&sh.raw_full[t & 1][0], t >> 1);
+        } else {
+          asm volatile("cp.async.wait_group 2;" ::: "memory");
         }
+        loader.convert(t, raw, k_dst, load_tid);
       }
       to_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.k_full[kb]);
+      if constexpr (S::kRaw) {  // everybody has read the raw bytes
+        asm volatile("bar.sync 2, 96;" ::: "memory");
+        if (load_tid == 0) loader.fetch_raw(false, t + 2, raw);
+      }
       // values: the buffer is free once the outputs that read it are there
       if (KV != kKvF16 && v_use > 0) wait(&sh.v_empty[vb], v_use - 1);
       if constexpr (KV == kKvF32) {
-        loader.split_rows(true, t, v_dst, load_tid);
+        loader.split_rows(true, t, raw_s, v_dst, load_tid);
       } else {
-        if constexpr (S::kRaw) asm volatile("cp.async.wait_group 3;" ::: "memory");
+        if constexpr (S::kRaw) wait(&sh.raw_full[t & 1][1], t >> 1);
         else asm volatile("cp.async.wait_group 1;" ::: "memory");
         loader.convert(t, raw + S::kRawBytes, v_dst, load_tid);
-        if constexpr (S::kRaw) loader.fetch(true, t + 2, raw + S::kRawBytes, load_tid);
       }
       to_async_proxy();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.v_full[vb]);
+      if constexpr (S::kRaw) {
+        asm volatile("bar.sync 2, 96;" ::: "memory");
+        if (load_tid == 0) loader.fetch_raw(true, t + 2, raw + S::kRawBytes);
+      }
       if constexpr (KV == kKvF16) {
         // The next tile's values and the keys of the one after it, straight into their buffers.  (The values of this tile's
         // buffer are in use until the scores of the next tile have been issued, for which its keys have to be published first.)
@@ -857,26 +902,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!ok) {  // bulk copies may be under way still: a millisecond for them
+      const long long begin = clock64();
+      while (clock64() - begin < 2000000) {
+      }
+    }
   } else if (lane == 0) {
     const uint32_t s_shape = tc_shape(kTcKeys, false), o_shape = tc_shape(128, true);
     auto scores = [&](int t) {
       const uint32_t d = tmem + kColS + (t & 1) * 64;
-      const uint32_t at = smem_u32(k_s + (t % S::kKBufs) * S::kTileBytes);
-#pragma unroll
+      const uint32_t at = smem_u32(k_s + (t % S::kBufs) * S::kTileBytes);
+#pragma unroll 4
       for (int kk = 0; kk < D / 16; ++kk) {  // the small products first
         const uint64_t b = tc_operand(at + kk * 256, 128, S::kGroupBytes);
         tc_mma(d, tmem + kColQ + D / 2 + kk * 8, b, s_shape, kk != 0);
         if (S::kTerms == 2) tc_mma(d, tmem + kColQ + kk * 8, tc_operand(at + S::kTermBytes + kk * 256, 128, S::kGroupBytes), s_shape, 1);
       }
-#pragma unroll
+#pragma unroll 4
       for (int kk = 0; kk < D / 16; ++kk)
         tc_mma(d, tmem + kColQ + kk * 8, tc_operand(at + kk * 256, 128, S::kGroupBytes), s_shape, 1);
       tc_commit(&sh.s_full[t & 1]);
-      tc_commit(&sh.k_empty[t % S::kKBufs]);
+      tc_commit(&sh.k_empty[t % S::kBufs]);
     };
     auto outputs = [&](int t, int h) {
       const uint32_t w = tmem + kColS + (t & 1) * 64;
-      const uint32_t at = smem_u32(v_s + (t % S::kVBufs) * S::kTileBytes) + h * 2048;
+      const uint32_t at = smem_u32(v_s + (t % S::kBufs) * S::kTileBytes) + h * 2048;
 #pragma unroll
       for (int kk = 0; kk < kTcKeys / 16; ++kk) {
         const uint64_t b = tc_operand(at + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128);
@@ -887,11 +937,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       for (int kk = 0; kk < kTcKeys / 16; ++kk)
         tc_mma(tmem + kColO, w + kk * 8, tc_operand(at + kk * 2 * S::kGroupBytes, S::kGroupBytes, 128), o_shape, 1);
       tc_commit(&sh.o_full);
-      if (h == S::kHalves - 1) tc_commit(&sh.v_empty[t % S::kVBufs]);
+      if (h == S::kHalves - 1) tc_commit(&sh.v_empty[t % S::kBufs]);
     };
     auto next_scores = [&](int t) {
       if (t >= tiles) return;
-      wait(&sh.k_full[t % S::kKBufs], t / S::kKBufs);
+      wait(&sh.k_full[t % S::kBufs], t / S::kBufs);
       tc_after();
       if (ok) scores(t);
     };
@@ -900,7 +950,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     for (int t = 0; t < tiles && ok; ++t) {
       // outputs of a half: the weights and values are there, and the half before has been read
       wait(&sh.p_full[t & 1], t >> 1);
-      wait(&sh.v_full[t % S::kVBufs], t / S::kVBufs);
+      wait(&sh.v_full[t % S::kBufs], t / S::kBufs);
 #pragma unroll
       for (int h = 0; h < S::kHalves; ++h) {
         if (t + h > 0) wait(&sh.o_read, S::kHalves * t + h - 1);
@@ -921,25 +971,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
   if (warp == kTcThreads / 32 - 1) tc_free(tmem);
 }
 
-// The chunks of a (row, head), a thread four elements; zero where no chunk had a key.
-__global__ void __launch_bounds__(256)
+// The chunks of a (row, head), at most 64, by a warp; zero where no chunk had a key.
+constexpr int kMergeWarps = 4, kMostSplits = 64;
+template <int D>
+__global__ void __launch_bounds__(kMergeWarps * 32)
 attention_tree_merge_kernel(const float* __restrict__ pacc, const float* __restrict__ pmax, const float* __restrict__ psum,
-                            float* __restrict__ out, int dim4, int splits, size_t total) {
-  const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (t >= total) return;
-  const size_t row = t / dim4, e = t - row * dim4, base = row * splits;
-  float top = kNoKey, den = 0.0f;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, pmax[base + s]);
-  float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+                            float* __restrict__ out, int splits, int total) {
+  const int lane = threadIdx.x & 31;
+  const size_t row = static_cast<size_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+  if (row >= static_cast<size_t>(total)) return;
+  const size_t base = row * splits;
+  float top[2], sum[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int s = lane + 32 * u;
+    top[u] = s < splits ? pmax[base + s] : kNoKey, sum[u] = s < splits ? psum[base + s] : 0.0f;
+  }
+  float most = fmaxf(top[0], top[1]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+  const float w[2] = {exp2f(top[0] - most), exp2f(top[1] - most)};
+  const float den = warp_sum(fmaf(w[0], sum[0], w[1] * sum[1]));
+  float4 num[D / 128];
+#pragma unroll
+  for (int k = 0; k < D / 128; ++k) num[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4* src = reinterpret_cast<const float4*>(pacc) + base * (D / 4) + lane;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
-    const float w = exp2f(pmax[base + s] - top);
-    const float4 x = reinterpret_cast<const float4*>(pacc)[(base + s) * dim4 + e];
-    den = fmaf(w, psum[base + s], den);
-    num.x = fmaf(w, x.x, num.x), num.y = fmaf(w, x.y, num.y), num.z = fmaf(w, x.z, num.z), num.w = fmaf(w, x.w, num.w);
+    const float ws = __shfl_sync(0xFFFFFFFFu, s < 32 ? w[0] : w[1], s & 31);
+#pragma unroll
+    for (int k = 0; k < D / 128; ++k) {
+      const float4 x = __ldcs(src + s * (D / 4) + k * 32);
+      num[k].x = fmaf(ws, x.x, num[k].x), num[k].y = fmaf(ws, x.y, num[k].y), num[k].z = fmaf(ws, x.z, num[k].z), num[k].w = fmaf(ws, x.w, num[k].w);
+    }
   }
   const float f = den == 0.0f ? 0.0f : 1.0f / den;
-  reinterpret_cast<float4*>(out)[t] = make_float4(num.x * f, num.y * f, num.z * f, num.w * f);
+#pragma unroll
+  for (int k = 0; k < D / 128; ++k)
+    reinterpret_cast<float4*>(out)[row * (D / 4) + k * 32 + lane] = make_float4(num[k].x * f, num[k].y * f, num[k].z * f, num[k].w * f);
 }
 
 template <int KV, int D>
@@ -948,11 +1017,19 @@ int launch_tree_tc(TcParams p, cudaStream_t st) {
   static_assert(S::kSmem + sizeof(TcShared) <= 227 * 1024, "shared memory of a CTA");
   const auto kernel = attention_tree_tc_kernel<KV, D>;
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), S::kSmem)) return rc;
+  CUtensorMap maps[2] = {};
+  if (S::kRaw) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.t.kv_heads) * S::kRowBytes, static_cast<uint64_t>(p.t.n) + p.t.m}, stride = dims[0];
+    const uint32_t box[2] = {S::kBox, kTcKeys};
+    for (int i = 0; i < 2; ++i)
+      if (int rc = encode_tensor_map(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i ? p.t.v : p.t.k, dims, &stride, box, S::kBox == 128)) return rc;
+  }
   const dim3 grid(static_cast<unsigned>(p.t.kv_heads * p.row_tiles), static_cast<unsigned>(p.splits));
-  kernel<<<grid, kTcThreads, S::kSmem, st>>>(p);
+  kernel<<<grid, kTcThreads, S::kSmem, st>>>(maps[0], maps[1], p);
   if (int rc = check_launch(); rc != kOk || p.pacc == nullptr) return rc;
-  const size_t total = static_cast<size_t>(p.t.m) * p.t.heads * D / 4;
-  attention_tree_merge_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, st>>>(p.pacc, p.pmax, p.psum, p.t.out, D / 4, p.splits, total);
+  const int total = p.t.m * p.t.heads;
+  attention_tree_merge_kernel<D><<<static_cast<unsigned>((total + kMergeWarps - 1) / kMergeWarps), kMergeWarps * 32, 0, st>>>(p.pacc, p.pmax, p.psum, p.t.out,
+                                                                                                                        p.splits, total);
   return check_launch();
 }
 
@@ -982,7 +1059,7 @@ int launch_tree(const TreeParams& t, uint64_t head_dim, cudaStream_t st) {
   }();
   long best_splits = 1;
   double best = 0.0;
-  for (long s = 1; s <= 64 && s <= tiles; ++s) {
+  for (long s = 1; s <= kMostSplits && s <= tiles; ++s) {
     const long per = (tiles + s - 1) / s;
     if ((tiles + per - 1) / per != s) continue;
     const double waves = static_cast<double>((units * s + sms - 1) / sms);
