@@ -176,6 +176,7 @@ struct TcShared {
   float weighed[2][kTcRows];                        // the same of score + log2 of the value's scale
   uint32_t q_most[2][kTcRows];
   float sum[2][kTcRows];
+  int to[kTcRows], bad[kTcRows], any_bad;           // (bad: something that is not finite)
 };
 
 __device__ __forceinline__ void tc_alloc(uint32_t* slot) {
@@ -499,32 +500,38 @@ struct TcLoader {
       for (int u = 0; u < S::kRun; ++u)
 #pragma unroll
         for (int i = 0; i < kPer; ++i) x[u][i] = *reinterpret_cast<const float4*>(src + u * S::kRowBytes + i * 512);
+      uint32_t most[S::kRun];
 #pragma unroll
       for (int u = 0; u < S::kRun; ++u) {
-        const int key = (b * S::kRun + u) * kLoadWarps + warp;
-        if (key >= kTcKeys) break;
-        uint32_t most = 0;
-        const bool zero = unseen(min(c0 + t * kTcKeys + key, c1 - 1));
+        const int key = (b * S::kRun + u) * kLoadWarps + warp, j = min(c0 + t * kTcKeys + key, c1 - 1);
+        const bool zero = key >= kTcKeys || (j >= p.t.n && unseen(j));
+        most[u] = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           if (zero) x[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          most = max(max(most, max(__float_as_uint(x[u][i].x) & 0x7FFFFFFFu, __float_as_uint(x[u][i].y) & 0x7FFFFFFFu)),
-                     max(__float_as_uint(x[u][i].z) & 0x7FFFFFFFu, __float_as_uint(x[u][i].w) & 0x7FFFFFFFu));
+          most[u] = max(max(most[u], max(__float_as_uint(x[u][i].x) & 0x7FFFFFFFu, __float_as_uint(x[u][i].y) & 0x7FFFFFFFu)),
+                        max(__float_as_uint(x[u][i].z) & 0x7FFFFFFFu, __float_as_uint(x[u][i].w) & 0x7FFFFFFFu));
         }
-        most = __reduce_max_sync(0xFFFFFFFFu, most);
-        const int e = most == 0 ? 0 : max(-110, min(114, static_cast<int>(most >> 23) - 127 - 13));
-        const float up = power_of_two(-e);
-        if (most != 0) high = max(high, e), low = min(low, e);
-        if (lane == 0) sh.scale[t % kScaleBufs][values ? 1 : 0][key] = power_of_two(e);
+      }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          uint2 hi, lo;
-          tree_split(x[u][i].x * up, x[u][i].y * up, hi.x, lo.x);
-          tree_split(x[u][i].z * up, x[u][i].w * up, hi.y, lo.y);
-          const int c = i * 16 + lane / 2;
-          unsigned char* at = dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + c * 128 + (lane & 1) * 8;
-          *reinterpret_cast<uint2*>(at) = hi;
-          *reinterpret_cast<uint2*>(at + S::kTermBytes) = lo;
+      for (int u = 0; u < S::kRun; ++u) most[u] = __reduce_max_sync(0xFFFFFFFFu, most[u]);
+#pragma unroll
+      for (int u = 0; u < S::kRun; ++u) {
+        const int key = (b * S::kRun + u) * kLoadWarps + warp;
+        const int e = most[u] == 0 ? 0 : max(-110, min(114, static_cast<int>(most[u] >> 23) - 127 - 13));
+        const float up = power_of_two(-e);
+        if (most[u] != 0) high = max(high, e), low = min(low, e);
+        if (key < kTcKeys) {
+          if (lane == 0) sh.scale[t % kScaleBufs][values ? 1 : 0][key] = power_of_two(e);
+          unsigned char* at = dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + lane / 2 * 128 + (lane & 1) * 8;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            uint2 hi, lo;
+            tree_split(x[u][i].x * up, x[u][i].y * up, hi.x, lo.x);
+            tree_split(x[u][i].z * up, x[u][i].w * up, hi.y, lo.y);
+            *reinterpret_cast<uint2*>(at + i * 2048) = hi;
+            *reinterpret_cast<uint2*>(at + i * 2048 + S::kTermBytes) = lo;
+          }
         }
       }
       ask_rows(s + S::kRuns, ring, tid);
@@ -569,8 +576,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
   TcLoader<KV, D> loader{p, sh, &k_map, &v_map, kv, c0, c1, tiles};
 
   if (tid < kTreeWords) sh.used[tid] = 0;
+  if (tid < kTcRows) sh.bad[tid] = 0;
   if (tid < p.t.m) sh.parents[tid] = p.t.parents[tid];
   if (tid == 0) {
+    sh.any_bad = 0;
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sh.k_full[b], kLoadThreads / 32), mbar_init(&sh.v_full[b], kLoadThreads / 32);
       mbar_init(&sh.k_empty[b], 1), mbar_init(&sh.v_empty[b], 1);
@@ -811,39 +820,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
       unit = next_unit;
     }
     take_tile(tiles - 1);
-    // Through shared memory (the operands' buffers are free), so that a warp writes whole rows.
-    sh.sum[half][row] = sum;
+    // Through shared memory (the operands' buffers are free), so that a warp writes whole rows.  A NaN or an infinity among a
+    // row's operands has made its sums so (that of a key which it does not see as well: its weight of 0 does not mask it).
+    float all = sum;
 #pragma unroll
     for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-      for (int c = 0; c < 64; c += 4)
+      for (int c = 0; c < 64; c += 4) {
+        all = fmaf((o[h][c] + o[h][c + 1]) + (o[h][c + 2] + o[h][c + 3]), 0.0f, all);
         *reinterpret_cast<float4*>(smem + row * (D * 4) + (((h * 32 + half * 16 + c / 4) ^ (row & 7)) << 4)) =
             make_float4(o[h][c], o[h][c + 1], o[h][c + 2], o[h][c + 3]);
-    if (half == 0) sh.top[0][0][row] = mx;
+      }
+    sh.sum[half][row] = sum;
+    if (half == 0) {
+      sh.top[0][0][row] = mx;
+      sh.to[row] = tree_i * p.t.heads + kv * p.group + (row0 + row) - tree_i * p.group;  // its (row, head)
+    }
+    if (row < rows && !(fabsf(all) <= 3.402823466e38f)) sh.bad[row] = sh.any_bad = 1;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-#pragma unroll 1
+#pragma unroll 4
     for (int r = warp; r < rows; r += kSoftThreads / 32) {
-      const int i = (row0 + r) / p.group;
-      const size_t at = static_cast<size_t>(i) * p.t.heads + kv * p.group + (row0 + r) - i * p.group;
+      const size_t at = static_cast<size_t>(sh.to[r]);
       const float total = sh.sum[0][r] + sh.sum[1][r], f = p.pacc != nullptr ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
       float4* dst = reinterpret_cast<float4*>(p.pacc != nullptr ? p.pacc + (at * p.splits + split) * D : p.t.out + at * D);
-      float all = total;
-      float4 y[D / 128];
+      const bool bad = sh.bad[r] != 0;
 #pragma unroll
       for (int k = 0; k < D / 128; ++k) {
-        y[k] = *reinterpret_cast<const float4*>(smem + r * (D * 4) + (((k * 32 + lane) ^ (r & 7)) << 4));
-        all = fmaf((y[k].x + y[k].y) + (y[k].z + y[k].w), 0.0f, all);
+        const float4 y = *reinterpret_cast<const float4*>(smem + r * (D * 4) + (((k * 32 + lane) ^ (r & 7)) << 4));
+        if (!bad) dst[k * 32 + lane] = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
       }
-      // A NaN or an infinity among a row's operands has made its sums so (that of a key which it does not see as well: its weight
-      // of 0 does not mask it).
-      if (!__all_sync(0xFFFFFFFFu, fabsf(all) <= 3.402823466e38f)) {
-        tree_scalar_row<KV, D>(p, sh, kv, row0 + r, c0, c1, split);
-        continue;
-      }
-#pragma unroll
-      for (int k = 0; k < D / 128; ++k) dst[k * 32 + lane] = make_float4(y[k].x * f, y[k].y * f, y[k].z * f, y[k].w * f);
-      if (p.pacc != nullptr && lane == 0) p.pmax[at * p.splits + split] = sh.top[0][0][r], p.psum[at * p.splits + split] = total;
+      if (p.pacc != nullptr && lane == 0 && !bad) p.pmax[at * p.splits + split] = sh.top[0][0][r], p.psum[at * p.splits + split] = total;
     }
+    if (sh.any_bad != 0)
+      for (int r = warp; r < rows; r += kSoftThreads / 32)
+        if (sh.bad[r] != 0) tree_scalar_row<KV, D>(p, sh, kv, row0 + r, c0, c1, split);
   } else if (loading) {
     float k_next = 0.0f, v_next = 0.0f;  // the next tile's scales
     if (S::kRaw) loader.next_scales(0, load_tid, k_next, v_next);
@@ -977,6 +987,7 @@ template <int D>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 attention_tree_merge_kernel(const float* __restrict__ pacc, const float* __restrict__ pmax, const float* __restrict__ psum,
                             float* __restrict__ out, int splits, int total) {
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const size_t row = static_cast<size_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
   if (row >= static_cast<size_t>(total)) return;
@@ -1028,8 +1039,12 @@ int launch_tree_tc(TcParams p, cudaStream_t st) {
   kernel<<<grid, kTcThreads, S::kSmem, st>>>(maps[0], maps[1], p);
   if (int rc = check_launch(); rc != kOk || p.pacc == nullptr) return rc;
   const int total = p.t.m * p.t.heads;
-  attention_tree_merge_kernel<D><<<static_cast<unsigned>((total + kMergeWarps - 1) / kMergeWarps), kMergeWarps * 32, 0, st>>>(p.pacc, p.pmax, p.psum, p.t.out,
-                                                                                                                        p.splits, total);
+  // (its launch overlaps the end of the chunks' kernel, which it waits for before it reads or writes anything)
+  if (launch_kernel(attention_tree_merge_kernel<D>, dim3(static_cast<unsigned>((total + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0, st, true,
+                    p.pacc, p.pmax, p.psum, p.t.out, p.splits, total) != cudaSuccess) {
+    cudaGetLastError();
+    return kDeviceError;
+  }
   return check_launch();
 }
 
