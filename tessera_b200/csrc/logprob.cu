@@ -40,14 +40,22 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 }
 __device__ __forceinline__ Entry64 entry_of(float x, uint32_t index) { return static_cast<Entry64>(order_of(x)) << 32 | (0xFFFFFFFFu - index); }
 
-struct Sums {  // of e^(x - top) and of e^(x - top) (x - top); top is -inf before the first finite logit
+// 2^x without the slow path below the normal numbers (0 there; its neighbours of a sum are 1 or more)
+__device__ __forceinline__ float power2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLpLog2e = 1.4426950408889634f, kLpLn2 = 0.6931471805599453f;
+struct Sums {  // y = (x - top) log2 e: sums of 2^y and of 2^y y; top is -inf before the first finite logit
   float top, s, t;
 };
 __device__ __forceinline__ float shift_of(float top) { return top == -INFINITY ? 0.0f : top; }
 __device__ __forceinline__ Sums moved(const Sums& a, float top) {  // top >= a.top
-  const float by = shift_of(a.top) - shift_of(top);
+  const float by = (shift_of(a.top) - shift_of(top)) * kLpLog2e;
   if (a.s == 0.0f) return Sums{top, a.s, a.t};  // (nothing so far; its top may be -inf)
-  const float f = exp2f(by * 1.4426950408889634f);
+  const float f = power2(by);
   return Sums{top, a.s * f, f == 0.0f ? 0.0f : f * fmaf(a.s, by, a.t)};  // (by may be -inf: logits of the type's lowest value)
 }
 __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
@@ -71,20 +79,23 @@ struct LogprobShared {
   Sums sums[kLpWarps], all;
   uint32_t bound[kLpWarps];
   int count;
-  int had;  // entries before the tile at hand (fewer than kLpCut)
 };
 
-// The list's top_k largest to its front, in order; returns the entry that a new one has to exceed (0: none).
+// The list's top_k largest to its front, in order; returns the entry that a new one has to exceed (0: none).  Several threads
+// count for an entry where there are few.
 __device__ __forceinline__ Entry64 cut_back(LogprobShared& sh, int n, int top_k) {
   const int tid = threadIdx.x;
-#pragma unroll
-  for (int r = 0; r < kLpList / kLpThreads; ++r) {
-    const int i = tid + r * kLpThreads;
-    if (i >= n) break;
-    const Entry64 mine = sh.list[i];
+  int log = 0;  // 2^log threads an entry
+  while (log < 5 && (n << (log + 1)) <= kLpThreads) ++log;
+  const int part = tid & ((1 << log) - 1);
+  for (int i0 = 0; i0 < n; i0 += kLpThreads >> log) {
+    const int i = i0 + (tid >> log);
+    const Entry64 mine = sh.list[min(i, n - 1)];
     int above = 0;
-    for (int j = 0; j < n; ++j) above += sh.list[j] > mine ? 1 : 0;
-    if (above < top_k) sh.cut[above] = mine;
+#pragma unroll 8
+    for (int j = part; j < n; j += 1 << log) above += sh.list[j] > mine ? 1 : 0;
+    for (int o = 1; o < 1 << log; o <<= 1) above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
+    if (part == 0 && i < n && above < top_k) sh.cut[above] = mine;
   }
   __syncthreads();
   const int left = min(n, top_k);
@@ -124,7 +135,7 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
       }
     }
   };
-  if (tid == 0) sh.count = sh.had = 0;
+  if (tid == 0) sh.count = 0;
   load(begin);
   Sums mine{-INFINITY, 0.0f, 0.0f};
   Entry64 least = 0;             // a new entry has to exceed it
@@ -141,12 +152,14 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
     for (int i = 1; i < kLpPer; ++i) most = fmaxf(most, v[i]);
     if (most > mine.top) mine = moved(mine, most);
     const float shift = shift_of(mine.top);
+    float s[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kLpPer; ++i) {
-      const float y = v[i] - shift, e = exp2f(y * 1.4426950408889634f);
-      mine.s += e;
-      mine.t = fmaf(e, fmaxf(y, -1e30f), mine.t);  // a masked logit is 0 * -1e30
+      const float y = (v[i] - shift) * kLpLog2e, e = power2(y);
+      s[i & 1] += e;
+      u[i & 1] = fmaf(e, fmaxf(y, -1e30f), u[i & 1]);  // a masked logit is 0 * -1e30
     }
+    mine.s += s[0] + s[1], mine.t += u[0] + u[1];
     if (top_k == 0) continue;
     if (tile == begin) {
       // The full[] warps whose every lane holds logits each give the per_warp-th largest of their lanes' maxima: at least
@@ -169,67 +182,69 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
       least = bound == 0 ? 0 : static_cast<Entry64>(bound) << 32;
       threshold = bound == 0 ? -INFINITY : value_of(bound);
     }
-    uint32_t above = 0;
+    // The few logits that reach the threshold.  (A NaN is above nothing: it comes up only while there is no threshold.)
+    int last_slot = -1;
+    if (!(most < threshold)) {
+      uint32_t above = 0;
 #pragma unroll
-    for (int i = 0; i < kLpPer; ++i)
-      if (!(v[i] < threshold)) above |= 1u << i;
-    if (above != 0) {
+      for (int i = 0; i < kLpPer; ++i)
+        if (!(v[i] < threshold)) above |= 1u << i;
+#pragma unroll 1
+      for (; above != 0; above &= above - 1) {
+        const int which = __ffs(above) - 1;
+        float value = v[0];
 #pragma unroll
-      for (int i = 0; i < kLpPer; ++i) {
-        const uint32_t at = index_of(tile, i);
-        if ((above >> i & 1u) && (at >= end || entry_of(v[i], at) <= least)) above &= ~(1u << i);
-      }
-      if (above != 0) {
-        int slot = atomicAdd(&sh.count, __popc(above));
-#pragma unroll
-        for (int i = 0; i < kLpPer; ++i)
-          if (above >> i & 1u) {
-            if (slot < kLpList) sh.list[slot] = entry_of(v[i], index_of(tile, i));
-            ++slot;
-          }
+        for (int i = 1; i < kLpPer; ++i) value = which == i ? v[i] : value;
+        const uint32_t at = index_of(tile, which);
+        const Entry64 e = entry_of(value, at);
+        if (at >= end || e <= least) continue;
+        last_slot = atomicAdd(&sh.count, 1);
+        if (last_slot < kLpList) sh.list[last_slot] = e;
       }
     }
-    __syncthreads();
+    const bool last = tile + kLpTile >= end;
+    if (!__syncthreads_or(last_slot >= kLpCut - 1) && tile != begin && !last) continue;
     int n = sh.count;
     if (n > kLpList) {
-      // The list overflowed: its first entries are the ones it had, at most kLpCut; what this tile added is found again.
-      // Bisection for the top_k-th largest entry of both.
-      const int had = sh.had;
+      // The list overflowed.  Its first entries, fewer than kLpCut, are those of the tiles before; this tile's are found again:
+      // bisection for the top_k-th largest entry of both.
+      __syncthreads();
+      const Entry64 kept = tid < kLpCut ? sh.list[tid] : 0;
+      const uint32_t where = 0xFFFFFFFFu - static_cast<uint32_t>(kept);
+      const bool before = tid < kLpCut && (where < tile || where >= tile + kLpTile);
       Entry64 lo = 0;
       for (int bit = 63; bit >= 0; --bit) {
         const Entry64 trial = lo | (1ull << bit);
-        int mine_above = tid < had && sh.list[tid] >= trial ? 1 : 0;
-#pragma unroll
-        for (int i = 0; i < kLpPer; ++i)
-          if ((above >> i & 1u) && entry_of(v[i], index_of(tile, i)) >= trial) ++mine_above;
         if (tid == 0) sh.count = 0;
         __syncthreads();
+        int mine_above = before && kept >= trial ? 1 : 0;
+#pragma unroll
+        for (int i = 0; i < kLpPer; ++i) {
+          const uint32_t at = index_of(tile, i);
+          const Entry64 e = entry_of(v[i], at);
+          if (at < end && e > least && e >= trial) ++mine_above;
+        }
         mine_above = __reduce_add_sync(0xFFFFFFFFu, mine_above);
         if (lane == 0 && mine_above != 0) atomicAdd(&sh.count, mine_above);
         __syncthreads();
         if (sh.count >= top_k) lo = trial;
         __syncthreads();
       }
-      Entry64 kept = 0;
-      if (tid < had) kept = sh.list[tid];
       if (tid == 0) sh.count = 0;
       __syncthreads();
-      if (tid < had && kept >= lo) sh.list[atomicAdd(&sh.count, 1)] = kept;
-#pragma unroll
+      if (before && kept >= lo) sh.list[atomicAdd(&sh.count, 1)] = kept;
+#pragma unroll 1
       for (int i = 0; i < kLpPer; ++i) {
-        const Entry64 e = entry_of(v[i], index_of(tile, i));
-        if ((above >> i & 1u) && e >= lo) sh.list[atomicAdd(&sh.count, 1)] = e;
+        const uint32_t at = index_of(tile, i);
+        if (at >= end) continue;
+        const Entry64 e = entry_of(x[at], at);
+        if (e > least && e >= lo) sh.list[atomicAdd(&sh.count, 1)] = e;
       }
       __syncthreads();
       n = sh.count;
     }
-    if (tile == begin || n >= kLpCut || tile + kLpTile >= end) {
-      const Entry64 cut = cut_back(sh, n, top_k);
-      if (cut != 0) least = cut, threshold = value_of(static_cast<uint32_t>(cut >> 32));
-      n = min(n, top_k);
-    }
-    if (tid == 0) sh.had = n;
-    __syncthreads();
+    const Entry64 cut = cut_back(sh, n, top_k);
+    if (cut != 0) least = cut, threshold = value_of(static_cast<uint32_t>(cut >> 32));
   }
 
   // the threads' sums, then the CTAs'
@@ -284,7 +299,7 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
   if (tid == 0) {
     const uint32_t t = targets[row];
     logprob[row] = nothing || t >= vocab ? (all.s == all.s ? -INFINITY : all.s) : (x[t] - top) - log_s;
-    entropy[row] = nothing ? 0.0f : log_s - all.t / all.s;
+    entropy[row] = nothing ? 0.0f : log_s - all.t / all.s * kLpLn2;
   }
   if (tid < top_k) {
     const Entry64 e = sh.list[tid];
