@@ -14,6 +14,8 @@
 // equal logits) finds its own threshold by bisection over the entries.  The CTAs meet through distributed shared memory.
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "codec.cuh"
 #include "launch.h"
 #include "tessera_b200.h"
@@ -21,12 +23,13 @@
 namespace tsr {
 namespace {
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32;
-constexpr int kLpPer = 16, kLpTile = kLpThreads * kLpPer;
-constexpr int kLpList = 1024;  // entries of the list: two a thread when it is cut back
-constexpr int kLpTop = 32;     // top_k at most, as top_k_rows
-constexpr int kLpCluster = 8;  // CTAs of a row at most (the portable cluster size)
-constexpr int kLpCut = 192;    // entries from which the list is cut back before the next tile
+constexpr int kLpMost = 512;    // threads of a CTA at most
+constexpr int kLpPer = 16;      // logits of a thread at a time
+constexpr int kLpList = 1024;   // entries of the list
+constexpr int kLpTop = 32;      // top_k at most, as top_k_rows
+constexpr int kLpCluster = 16;  // CTAs of a row at most
+constexpr int kLpCut = 96;      // entries from which the list is cut back before the next tile
+static_assert(kLpCluster * kLpTop <= kLpMost && kLpCut > kLpTop, "a thread an entry where the CTAs meet");
 
 using Entry64 = unsigned long long;
 
@@ -58,10 +61,18 @@ __device__ __forceinline__ Sums moved(const Sums& a, float top) {  // top >= a.t
   const float f = power2(by);
   return Sums{top, a.s * f, f == 0.0f ? 0.0f : f * fmaf(a.s, by, a.t)};  // (by may be -inf: logits of the type's lowest value)
 }
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-  const float top = fmaxf(a.top, b.top);
-  const Sums x = moved(a, top), y = moved(b, top);
-  return Sums{top, x.s + y.s, x.t + y.t};
+// Of a warp's lanes, in every lane.
+__device__ __forceinline__ Sums warp_joined(Sums a) {
+  float top = a.top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  a = moved(a, top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xFFFFFFFFu, a.s, o);
+    a.t += __shfl_xor_sync(0xFFFFFFFFu, a.t, o);
+  }
+  return a;
 }
 
 __device__ __forceinline__ uint32_t shared_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -75,25 +86,40 @@ __device__ __forceinline__ void cluster_meet() {
 }
 
 struct LogprobShared {
-  Entry64 list[kLpList], cut[kLpTop];
-  Sums sums[kLpWarps], all;
-  uint32_t bound[kLpWarps];
+  alignas(16) Entry64 list[kLpList + 256];
+  Entry64 cut[kLpTop];
+  Sums sums[kLpMost / 32], all;
+  uint32_t bound[kLpMost / 32];
   int count;
 };
 
+// (Named by both functions below: an address handed to one that is not inlined would be a generic one.)
+extern __shared__ __align__(16) unsigned char logprob_smem[];
+__device__ __forceinline__ LogprobShared& logprob_shared() { return *reinterpret_cast<LogprobShared*>(logprob_smem); }
+
 // The list's top_k largest to its front, in order; returns the entry that a new one has to exceed (0: none).  Several threads
 // count for an entry where there are few.
-__device__ __forceinline__ Entry64 cut_back(LogprobShared& sh, int n, int top_k) {
+template <int THREADS>
+__device__ __noinline__ Entry64 cut_back(int n, int top_k) {
+  LogprobShared& sh = logprob_shared();
   const int tid = threadIdx.x;
   int log = 0;  // 2^log threads an entry
-  while (log < 5 && (n << (log + 1)) <= kLpThreads) ++log;
+  while (log < 5 && (n << (log + 1)) <= THREADS) ++log;
   const int part = tid & ((1 << log) - 1);
-  for (int i0 = 0; i0 < n; i0 += kLpThreads >> log) {
+  if (tid < 8 << log) sh.list[n + tid] = 0;  // (they are read eight a thread at a time)
+  __syncthreads();
+  for (int i0 = 0; i0 < n; i0 += THREADS >> log) {
     const int i = i0 + (tid >> log);
     const Entry64 mine = sh.list[min(i, n - 1)];
     int above = 0;
-#pragma unroll 8
-    for (int j = part; j < n; j += 1 << log) above += sh.list[j] > mine ? 1 : 0;
+#pragma unroll 1
+    for (int j = 2 * part; j < n; j += 8 << log) {
+      ulonglong2 e[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) e[u] = *reinterpret_cast<const ulonglong2*>(&sh.list[j + u * (2 << log)]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) above += (e[u].x > mine ? 1 : 0) + (e[u].y > mine ? 1 : 0);
+    }
     for (int o = 1; o < 1 << log; o <<= 1) above += __shfl_xor_sync(0xFFFFFFFFu, above, o);
     if (part == 0 && i < n && above < top_k) sh.cut[above] = mine;
   }
@@ -107,12 +133,13 @@ __device__ __forceinline__ Entry64 cut_back(LogprobShared& sh, int n, int top_k)
 }
 
 // grid: (cluster size, rows) in clusters along x
-template <int VEC>
-__global__ void __launch_bounds__(kLpThreads, 2)
+template <int VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict__ targets, float* __restrict__ logprob,
                     float* __restrict__ entropy, uint32_t* __restrict__ top_ids, float* __restrict__ top_logprobs, uint32_t vocab,
                     int top_k, size_t row_base) {
-  __shared__ LogprobShared sh;
+  constexpr int kWarps = THREADS / 32, kTile = THREADS * kLpPer;
+  LogprobShared& sh = logprob_shared();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = blockIdx.x, ranks = gridDim.x;
   const size_t row = blockIdx.y;
@@ -121,7 +148,7 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
   const uint32_t begin = min(vocab, rank * share), end = min(vocab, begin + share);
   constexpr int kRuns = kLpPer / VEC;
   float next[kLpPer];
-  auto index_of = [&](uint32_t tile, int i) { return tile + (i / VEC) * (kLpThreads * VEC) + tid * VEC + i % VEC; };
+  auto index_of = [&](uint32_t tile, int i) { return tile + (i / VEC) * (THREADS * VEC) + tid * VEC + i % VEC; };
   auto load = [&](uint32_t tile) {
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
@@ -135,18 +162,23 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
       }
     }
   };
-  if (tid == 0) sh.count = 0;
   load(begin);
+  if (tid == 0) sh.count = 0;
+  float given = -INFINITY;  // the target's logit
+  if (rank == 0 && tid == 0) {
+    const uint32_t target = targets[row];
+    if (target < vocab) given = x[target];
+  }
   Sums mine{-INFINITY, 0.0f, 0.0f};
   Entry64 least = 0;             // a new entry has to exceed it
   float threshold = -INFINITY;  // its logit
   __syncthreads();
-  for (uint32_t tile = begin; tile < end; tile += kLpTile) {
+  for (uint32_t tile = begin; tile < end; tile += kTile) {
     float v[kLpPer];
 #pragma unroll
     for (int i = 0; i < kLpPer; ++i) v[i] = next[i];
-    if (tile + kLpTile < end) load(tile + kLpTile);
-    const uint32_t held = min(end - tile, static_cast<uint32_t>(kLpTile));
+    if (tile + kTile < end) load(tile + kTile);
+    const uint32_t held = min(end - tile, static_cast<uint32_t>(kTile));
     float most = v[0];
 #pragma unroll
     for (int i = 1; i < kLpPer; ++i) most = fmaxf(most, v[i]);
@@ -164,7 +196,7 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
     if (tile == begin) {
       // The full[] warps whose every lane holds logits each give the per_warp-th largest of their lanes' maxima: at least
       // top_k logits are not below the least of these.
-      const uint32_t full = held / (32 * VEC) < kLpWarps ? held / (32 * VEC) : kLpWarps;
+      const uint32_t full = held / (32 * VEC) < kWarps ? held / (32 * VEC) : kWarps;
       uint32_t bound = 0;
       if (full != 0) {
         const int per_warp = (top_k + static_cast<int>(full) - 1) / static_cast<int>(full);
@@ -176,8 +208,7 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
         }
         if (lane == 0) sh.bound[warp] = bound;
         __syncthreads();
-        bound = sh.bound[0];
-        for (uint32_t w = 1; w < full; ++w) bound = min(bound, sh.bound[w]);
+        bound = __reduce_min_sync(0xFFFFFFFFu, lane < static_cast<int>(full) ? sh.bound[lane] : 0xFFFFFFFFu);
       }
       least = bound == 0 ? 0 : static_cast<Entry64>(bound) << 32;
       threshold = bound == 0 ? -INFINITY : value_of(bound);
@@ -202,8 +233,10 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
         if (last_slot < kLpList) sh.list[last_slot] = e;
       }
     }
-    const bool last = tile + kLpTile >= end;
-    if (!__syncthreads_or(last_slot >= kLpCut - 1) && tile != begin && !last) continue;
+    const bool last = tile + kTile >= end;
+    // (the bound will do for one more tile)
+    const bool cut_now = last || (tile == begin && end - tile > 2 * kTile);
+    if (!__syncthreads_or(last_slot >= kLpCut - 1) && !cut_now) continue;
     int n = sh.count;
     if (n > kLpList) {
       // The list overflowed.  Its first entries, fewer than kLpCut, are those of the tiles before; this tile's are found again:
@@ -211,7 +244,7 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
       __syncthreads();
       const Entry64 kept = tid < kLpCut ? sh.list[tid] : 0;
       const uint32_t where = 0xFFFFFFFFu - static_cast<uint32_t>(kept);
-      const bool before = tid < kLpCut && (where < tile || where >= tile + kLpTile);
+      const bool before = tid < kLpCut && (where < tile || where >= tile + kTile);
       Entry64 lo = 0;
       for (int bit = 63; bit >= 0; --bit) {
         const Entry64 trial = lo | (1ull << bit);
@@ -243,52 +276,67 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
       __syncthreads();
       n = sh.count;
     }
-    const Entry64 cut = cut_back(sh, n, top_k);
+    const Entry64 cut = cut_back<THREADS>(n, top_k);
     if (cut != 0) least = cut, threshold = value_of(static_cast<uint32_t>(cut >> 32));
   }
 
   // the threads' sums, then the CTAs'
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums other{__shfl_xor_sync(0xFFFFFFFFu, mine.top, o), __shfl_xor_sync(0xFFFFFFFFu, mine.s, o), __shfl_xor_sync(0xFFFFFFFFu, mine.t, o)};
-    mine = (lane & o) == 0 ? joined(mine, other) : joined(other, mine);
-  }
+  const Sums none{-INFINITY, 0.0f, 0.0f};
+  mine = warp_joined(mine);
   if (lane == 0) sh.sums[warp] = mine;
   __syncthreads();
-  if (tid == 0) {
-    Sums all = sh.sums[0];
-    for (int w = 1; w < kLpWarps; ++w) all = joined(all, sh.sums[w]);
-    sh.all = all;
+  if (warp == 0) {
+    mine = warp_joined(lane < kWarps ? sh.sums[lane] : none);
+    if (lane == 0) sh.all = mine;
   }
   if (ranks > 1) {
     cluster_meet();
-    if (rank == 0) {
-      if (tid == 0) {
-        Sums all = sh.all;
-        for (uint32_t r = 1; r < ranks; ++r) {
-          const uint32_t at = peer_at(shared_at(&sh.all), r);
-          Sums other;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.top) : "r"(at) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.s) : "r"(at + 4) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.t) : "r"(at + 8) : "memory");
-          all = joined(all, other);
-        }
-        sh.all = all;
-      }
-      if (tid >= top_k && tid < static_cast<int>(ranks) * top_k) {
-        const uint32_t r = tid / top_k, i = tid % top_k;
-        uint32_t n;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(peer_at(shared_at(&sh.count), r)) : "memory");
-        Entry64 e = 0;
-        if (i < n) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(e) : "r"(peer_at(shared_at(&sh.list[i]), r)) : "memory");
-        sh.list[tid] = e != 0 ? e : tid;  // below every entry, and no two alike
-      }
-      if (tid < top_k && tid >= sh.count) sh.list[tid] = tid;
-      __syncthreads();
-      if (top_k != 0) cut_back(sh, static_cast<int>(ranks) * top_k, top_k);
+    if (rank != 0) {
+      cluster_meet();  // this CTA's shared memory is read until here
+      return;
     }
-    cluster_meet();  // the others' shared memory is read until here
-    if (rank != 0) return;
+    if (warp == 0) {
+      Sums other = none;
+      if (lane < static_cast<int>(ranks)) {
+        const uint32_t at = peer_at(shared_at(&sh.all), lane);
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.top) : "r"(at) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.s) : "r"(at + 4) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.t) : "r"(at + 8) : "memory");
+      }
+      other = warp_joined(other);
+      if (lane == 0) sh.sums[0] = other;
+    }
+    // A thread an entry.  What is below the last of some CTA's full list is not among the row's top_k.
+    Entry64 least_of = 0;
+    if (lane < static_cast<int>(ranks) && top_k != 0) {
+      uint32_t n;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(peer_at(shared_at(&sh.count), lane)) : "memory");
+      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(least_of) : "r"(peer_at(shared_at(&sh.list[top_k - 1]), lane)) : "memory");
+      if (n < static_cast<uint32_t>(top_k)) least_of = 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Entry64 other = __shfl_xor_sync(0xFFFFFFFFu, least_of, o);
+      least_of = other > least_of ? other : least_of;
+    }
+    static_assert(THREADS >= kLpCluster * kLpTop, "one entry a thread");
+    Entry64 e = 0;
+    if (tid < static_cast<int>(ranks) * top_k) {
+      const uint32_t r = tid / top_k, i = tid % top_k;
+      uint32_t n;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(peer_at(shared_at(&sh.count), r)) : "memory");
+      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(e) : "r"(peer_at(shared_at(&sh.list[i]), r)) : "memory");
+      if (i >= n || e < least_of) e = 0;
+    }
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // (and not waited for: nobody reads this CTA's memory)
+    if (tid == 0) sh.all = sh.sums[0], sh.count = 0;
+    __syncthreads();
+    if (e != 0) sh.list[atomicAdd(&sh.count, 1)] = e;
+    __syncthreads();
+    if (top_k != 0) cut_back<THREADS>(sh.count, top_k);
+    if (tid < top_k && tid >= sh.count) sh.list[tid] = tid;  // below every entry, and no two alike: the row has fewer logits
+    __syncthreads();
   } else {
     if (tid < top_k && tid >= sh.count) sh.list[tid] = tid;
     __syncthreads();
@@ -297,30 +345,49 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
   const bool nothing = all.s == 0.0f;  // every logit is -inf
   const float log_s = logf(all.s), top = shift_of(all.top);
   if (tid == 0) {
-    const uint32_t t = targets[row];
-    logprob[row] = nothing || t >= vocab ? (all.s == all.s ? -INFINITY : all.s) : (x[t] - top) - log_s;
+    logprob[row] = all.s != all.s ? all.s : nothing ? -INFINITY : (given - top) - log_s;
     entropy[row] = nothing ? 0.0f : log_s - all.t / all.s * kLpLn2;
   }
   if (tid < top_k) {
     const Entry64 e = sh.list[tid];
-    const bool some = e >= kLpThreads;  // (a place without an entry holds its number: the row has fewer logits than top_k)
+    const bool some = e >= kLpMost;  // (a place without an entry holds its number: the row has fewer logits than top_k)
     top_ids[row * top_k + tid] = some ? 0xFFFFFFFFu - static_cast<uint32_t>(e) : 0u;
     top_logprobs[row * top_k + tid] = all.s != all.s ? all.s : !some || nothing ? -INFINITY : (value_of(static_cast<uint32_t>(e >> 32)) - top) - log_s;
   }
 }
 
-// CTAs of a row: as many as the machine has room for at two a SM, while each has half a tile.
-unsigned logprob_ctas(uint64_t rows, uint64_t vocab) {
-  unsigned ctas = 1;
-  while (ctas < kLpCluster && rows * ctas * 2 <= 296 && vocab / (ctas * 2) >= kLpTile / 2) ctas *= 2;
-  return ctas;
+template <int VEC, int THREADS>
+int launch_logprob(unsigned ctas, uint64_t rows, const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids,
+                   float* top_logprobs, uint64_t vocab, uint64_t top_k, uint64_t row_base, cudaStream_t st) {
+  const auto kernel = logprob_rows_kernel<VEC, THREADS>;
+  if (ctas > 8) {  // clusters beyond the portable size
+    static std::atomic<unsigned long long> allowed{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return kDeviceError;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if ((allowed.load() & bit) == 0) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        ctas = 8;
+      } else {
+        allowed.fetch_or(bit);
+      }
+    }
+  }
+  const cudaError_t e = launch_kernel_cluster(kernel, dim3(ctas, static_cast<unsigned>(rows)), dim3(THREADS), sizeof(LogprobShared), st, false, ctas, logits, targets, logprob,
+                                              entropy, top_ids, top_logprobs, static_cast<uint32_t>(vocab), static_cast<int>(top_k), row_base);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return kDeviceError;
+  }
+  return check_launch();
 }
 
 }  // namespace
 
 int logprob_rows(const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids,
                                 float* top_logprobs, uint64_t rows, uint64_t vocab, uint64_t top_k, uint64_t row_base, bool dry, cudaStream_t st) {
-  if (!logits || !targets || !logprob || !entropy || rows == 0 || rows > 65535 || vocab == 0 || vocab > 0x7FFFFFFFull - kLpTile || top_k > kLpTop ||
+  if (!logits || !targets || !logprob || !entropy || rows == 0 || rows > 65535 || vocab == 0 || vocab > 0x7FFFFFFFull - kLpMost * kLpPer || top_k > kLpTop ||
       row_base > 0x7FFFFFFFull || (top_k != 0 && (!top_ids || !top_logprobs)))
     return kInvalidArgument;
   struct {
@@ -339,18 +406,13 @@ int logprob_rows(const float* logits, const uint32_t* targets, float* logprob, f
       if (meet(out[i], out[j])) return kInvalidArgument;
   }
   if (dry) return kOk;
-  const unsigned ctas = logprob_ctas(rows, vocab);
-  const dim3 grid(ctas, static_cast<unsigned>(rows));
+  // CTAs of a row: while the machine has room for them (two a SM; clusters of sixteen, of which a GPC holds few, one a SM) and each
+  // has a quarter of a tile.
+  unsigned ctas = 1;
+  while (ctas < kLpCluster && rows * (ctas * 2) <= (ctas < 8 ? 296 : 148) && vocab / (ctas * 2) >= kLpMost * kLpPer / 4) ctas *= 2;
   const bool wide = vocab % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15u) == 0;
-  const cudaError_t e = wide ? launch_kernel_cluster(logprob_rows_kernel<4>, grid, dim3(kLpThreads), 0, st, false, ctas, logits, targets, logprob,
-                                                    entropy, top_ids, top_logprobs, static_cast<uint32_t>(vocab), static_cast<int>(top_k), row_base)
-                            : launch_kernel_cluster(logprob_rows_kernel<1>, grid, dim3(kLpThreads), 0, st, false, ctas, logits, targets, logprob,
-                                                    entropy, top_ids, top_logprobs, static_cast<uint32_t>(vocab), static_cast<int>(top_k), row_base);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return kDeviceError;
-  }
-  return check_launch();
+  return wide ? launch_logprob<4, kLpMost>(ctas, rows, logits, targets, logprob, entropy, top_ids, top_logprobs, vocab, top_k, row_base, st)
+              : launch_logprob<1, kLpMost>(ctas, rows, logits, targets, logprob, entropy, top_ids, top_logprobs, vocab, top_k, row_base, st);
 }
 
 }  // namespace tsr
