@@ -251,6 +251,8 @@ int umma_f8_wait_timeouts(unsigned int* count);
 int umma_f8_set_error_word(unsigned int* word);
 int tree_wait_timeouts(unsigned int* count);
 int tree_set_error_word(unsigned int* word);
+int delta_wait_timeouts(unsigned int* count);
+int delta_set_error_word(unsigned int* word);
 // ---- merged small steps of a token (forward_elementwise.cu, attention.cu): what the deferred queue issues
 // when it finds these steps side by side; each merged kernel repeats the single steps' arithmetic.
 // Linear-attention layer: ssm_gate, conv1d_state (one row, no history slots), l2norm of the q and k heads in
