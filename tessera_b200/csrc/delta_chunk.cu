@@ -145,21 +145,24 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
 // grid: (chunks, key heads), 8 warps.  Up to four value heads at a time: the substitution is a warp's, everything else is spread
 // over all warps.
 constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32, kPrepHeads = 4, kPitch = kChunk + 4;
+struct PrepHead {
+  float solve[kChunk][kPitch];  // the system, then T
+  float out[kChunk][kPitch];    // the decays G, then P
+};
 struct PrepShared {
-  float solve[kPrepHeads][kChunk][kPitch];  // the system, then T
-  float out[kPrepHeads][kChunk][kPitch];    // the decays G, then P
   float gram[2][kChunk][kPitch];            // k_t . k_s and q_t . k_s
   float fold[kPrepHeads][kChunk];           // g_s 2^e(k_s)
   float beta[kPrepHeads][kChunk];
   float unit[2][kChunk];
 };
-template <int DK>
-__global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(const DeltaChunkParams p) {
+template <int DK, int PER_SM>
+__global__ void __launch_bounds__(kPrepThreads, PER_SM) delta_chunk_prepare_kernel(const DeltaChunkParams p) {
   using S = ChunkShape<DK>;
   extern __shared__ __align__(128) unsigned char prep_smem[];
-  // K, Q and W as two terms, as in the workspace: bulk copies take them there
-  unsigned char *const op_s = prep_smem, *const w_s = prep_smem + 2 * S::kKeyBytes;
-  PrepShared& sh = *reinterpret_cast<PrepShared*>(prep_smem + 3 * S::kKeyBytes);
+  // K and Q as two terms, as in the workspace: bulk copies take them there; W takes Q's place
+  unsigned char *const op_s = prep_smem, *const w_s = prep_smem + S::kKeyBytes;
+  PrepShared& sh = *reinterpret_cast<PrepShared*>(prep_smem + 2 * S::kKeyBytes);
+  PrepHead* const hd = reinterpret_cast<PrepHead*>(prep_smem + 2 * S::kKeyBytes + sizeof(PrepShared));  // as many as there are, at most kPrepHeads
   pdl_trigger();  // (once every CTA has started, the scan's may)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int chunk = blockIdx.x, kh = blockIdx.y, t0 = chunk * kChunk, rows = min(kChunk, p.rows - t0), factor = p.heads / p.k_heads;
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
         decay = lane == t ? 1.0f : lane < t ? decay * a : 0.0f;
         start *= a;
         if (lane == t) mine = start;
-        sh.out[warp][t][lane] = decay;
+        hd[warp].out[t][lane] = decay;
       }
       Factors* const f = fac + warp * fac_step;
       f->query[lane] = mine * sh.unit[1][lane], f->put[lane] = decay * sh.unit[0][lane];
@@ -264,30 +267,29 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
     __syncthreads();
     for (int i = tid; i < heads * kChunk * kChunk / 4; i += kPrepThreads) {
       const int w = i / (kChunk * kChunk / 4), t = i / (kChunk / 4) % kChunk, s = i % (kChunk / 4) * 4;
-      const float4 d = *reinterpret_cast<const float4*>(&sh.out[w][t][s]), kk = *reinterpret_cast<const float4*>(&sh.gram[0][t][s]),
+      const float4 d = *reinterpret_cast<const float4*>(&hd[w].out[t][s]), kk = *reinterpret_cast<const float4*>(&sh.gram[0][t][s]),
                    qk = *reinterpret_cast<const float4*>(&sh.gram[1][t][s]);
       const float b = sh.beta[w][t];
-      *reinterpret_cast<float4*>(&sh.solve[w][t][s]) = make_float4(s < t ? b * d.x * kk.x : 0.0f, s + 1 < t ? b * d.y * kk.y : 0.0f,
+      *reinterpret_cast<float4*>(&hd[w].solve[t][s]) = make_float4(s < t ? b * d.x * kk.x : 0.0f, s + 1 < t ? b * d.y * kk.y : 0.0f,
                                                                    s + 2 < t ? b * d.z * kk.z : 0.0f, s + 3 < t ? b * d.w * kk.w : 0.0f);
-      *reinterpret_cast<float4*>(&sh.out[w][t][s]) =
+      *reinterpret_cast<float4*>(&hd[w].out[t][s]) =
           make_float4(s <= t ? d.x * qk.x : 0.0f, s + 1 <= t ? d.y * qk.y : 0.0f, s + 2 <= t ? d.z * qk.z : 0.0f, s + 3 <= t ? d.w * qk.w : 0.0f);
     }
     __syncthreads();
-    // values of u's warps: 32 columns, [16 columns][tile][row 2 t, 2 t + 1, + 8, ...], loaded a head ahead
-    float v[2][2][8];
+    // values of u's warps: 16 columns, [tile][row 2 t, 2 t + 1, + 8, ...], loaded ahead
+    float v[2][8];
     auto load_values = [&](int w, int c0) {
       const float* const src = p.v + (static_cast<size_t>(t0) * p.heads + kh + (f0 + w) * p.k_heads) * p.dv + c0 + g;
 #pragma unroll
-      for (int pair = 0; pair < 2; ++pair)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int s = (i >> 1) * 8 + 2 * t4 + (i & 1);
-            v[pair][e][i] = s < rows && c0 + 16 * pair < p.dv ? src[s * step_v + 16 * pair + 8 * e] : 0.0f;
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int s = (i >> 1) * 8 + 2 * t4 + (i & 1);
+          v[e][i] = s < rows && c0 < p.dv ? src[s * step_v + 8 * e] : 0.0f;
+        }
     };
-    if (warp >= 4) load_values(0, (warp - 4) * 32);
+    const int first = (warp - 4) * 16;
+    if (warp >= 4) load_values(0, first);
     if (warp < heads) {
       float x[kChunk];  // a column of the inverse
 #pragma unroll
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
         float sum[4] = {lane == t ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < (t + 3) / 4; ++s) {
-          const float4 row = *reinterpret_cast<const float4*>(&sh.solve[warp][t][4 * s]);
+          const float4 row = *reinterpret_cast<const float4*>(&hd[warp].solve[t][4 * s]);
           sum[0] = fmaf(-row.x, x[4 * s], sum[0]);
           if (4 * s + 1 < t) sum[1] = fmaf(-row.y, x[4 * s + 1], sum[1]);
           if (4 * s + 2 < t) sum[2] = fmaf(-row.z, x[4 * s + 2], sum[2]);
@@ -306,12 +308,12 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
       __syncwarp();
       const float b = sh.beta[warp][lane];
 #pragma unroll
-      for (int t = 0; t < kChunk; ++t) sh.solve[warp][t][lane] = x[t] * b;
+      for (int t = 0; t < kChunk; ++t) hd[warp].solve[t][lane] = x[t] * b;
       load_gates(f0 + kPrepHeads + warp);
     } else {  // P, eight lanes a row
       for (int i = (warp - heads) * 4 + (lane >> 3); i < heads * kChunk; i += (kPrepWarps - heads) * 4) {
         const int w = i / kChunk, t = i % kChunk, part = lane & 7;
-        const float4 x = *reinterpret_cast<const float4*>(&sh.out[w][t][4 * part]);
+        const float4 x = *reinterpret_cast<const float4*>(&hd[w].out[t][4 * part]);
         uint32_t most = quad_max(max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w))));
         most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 4));
         float up, unit;
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
             float2 y = make_float2(0.0f, 0.0f);
             const int s = step * 16 + 8 * c + 2 * t4;
             if (step <= m) {
-              y = *reinterpret_cast<const float2*>(&sh.solve[w][m * 16 + g + 8 * r][s]);
+              y = *reinterpret_cast<const float2*>(&hd[w].solve[m * 16 + g + 8 * r][s]);
               y.x *= sh.fold[w][s], y.y *= sh.fold[w][s + 1];
             }
             x[step][r][2 * c] = y.x, x[step][r][2 * c + 1] = y.y;
@@ -400,7 +402,7 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
         fence_async();
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (tid == 0) bulk_store(mats + w * mats_step, w_s, S::kKeyBytes);
-      } else {  // u: 32 columns a warp, all rows
+      } else {  // u: 16 columns a warp and turn, all rows
         // T as a right operand, rows 8 n + g; unit: what takes rows 8 n + 2 t, 2 t + 1 back
         uint32_t th[4][2][2], tl[4][2][2];
         float unit[4][2];
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
           for (int step = 0; step <= n / 2; ++step)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              y[step][c] = *reinterpret_cast<const float2*>(&sh.solve[w][8 * n + g][step * 16 + 8 * c + 2 * t4]);
+              y[step][c] = *reinterpret_cast<const float2*>(&hd[w].solve[8 * n + g][step * 16 + 8 * c + 2 * t4]);
               most = max(most, max(abs_bits(y[step][c].x), abs_bits(y[step][c].y)));
             }
           float up, mine;
@@ -424,45 +426,41 @@ __global__ void __launch_bounds__(kPrepThreads, 2) delta_chunk_prepare_kernel(co
             for (int c = 0; c < 2; ++c) two_terms(y[step][c].x * up, y[step][c].y * up, th[n][step][c], tl[n][step][c]);
         }
         float4* const u = p.u + static_cast<size_t>(kh + (f0 + w) * p.k_heads) * (p.dv / 16) * p.chunks * 128;
-        for (int c0 = (warp - 4) * 32; c0 < p.dv; c0 += 128) {
+#pragma unroll 1
+        for (int c0 = first; c0 < p.dv; c0 += 64) {
+          uint32_t ah[2][4], al[2][4];
+          float unit_c[2];
 #pragma unroll
-          for (int pair = 0; pair < 2; ++pair) {
-            if (c0 + 16 * pair >= p.dv) break;
-            const float(&x)[2][8] = v[pair];
-            uint32_t ah[2][4], al[2][4];
-            float unit_c[2];
+          for (int e = 0; e < 2; ++e) {
+            uint32_t most = 0;
+            float up;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = max(most, abs_bits(v[e][i]));
+            row_unit(quad_max(most), up, unit_c[e]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) two_terms(v[e][2 * i] * up, v[e][2 * i + 1] * up, ah[i >> 1][2 * (i & 1) + e], al[i >> 1][2 * (i & 1) + e]);
+          }
+          if (c0 + 64 < p.dv)
+            load_values(w, c0 + 64);
+          else if (w + 1 < heads)
+            load_values(w + 1, first);
+#pragma unroll
+          for (int n = 0; n < 4; n += 2) {
+            float hi[2][4] = {}, lo[2][4] = {};
+#pragma unroll
+            for (int step = 0; step <= n / 2; ++step) {
+              const uint32_t bh[4] = {th[n][step][0], th[n][step][1], th[n + 1][step][0], th[n + 1][step][1]};
+              const uint32_t bl[4] = {tl[n][step][0], tl[n][step][1], tl[n + 1][step][0], tl[n + 1][step][1]};
+              mma3(hi[0], hi[1], lo[0], lo[1], ah[step], al[step], bh, bl);
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              uint32_t most = 0;
-              float up;
+              float y[4];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) most = max(most, abs_bits(x[e][i]));
-              row_unit(quad_max(most), up, unit_c[e]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) two_terms(x[e][2 * i] * up, x[e][2 * i + 1] * up, ah[i >> 1][2 * (i & 1) + e], al[i >> 1][2 * (i & 1) + e]);
-            }
-#pragma unroll
-            for (int n = 0; n < 4; n += 2) {
-              float hi[2][4] = {}, lo[2][4] = {};
-#pragma unroll
-              for (int step = 0; step <= n / 2; ++step) {
-                const uint32_t bh[4] = {th[n][step][0], th[n][step][1], th[n + 1][step][0], th[n + 1][step][1]};
-                const uint32_t bl[4] = {tl[n][step][0], tl[n][step][1], tl[n + 1][step][0], tl[n + 1][step][1]};
-                mma3(hi[0], hi[1], lo[0], lo[1], ah[step], al[step], bh, bl);
-              }
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float y[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) y[c] = (hi[e][c] + lo[e][c]) * (unit[n + e][c & 1] * unit_c[c >> 1]);
-                u[(static_cast<size_t>(c0 / 16 + pair) * p.chunks + chunk) * 128 + (n + e) * 32 + lane] = make_float4(y[0], y[1], y[2], y[3]);
-              }
+              for (int c = 0; c < 4; ++c) y[c] = (hi[e][c] + lo[e][c]) * (unit[n + e][c & 1] * unit_c[c >> 1]);
+              u[(static_cast<size_t>(c0 / 16) * p.chunks + chunk) * 128 + (n + e) * 32 + lane] = make_float4(y[0], y[1], y[2], y[3]);
             }
           }
-          if (c0 + 128 < p.dv)
-            load_values(w, c0 + 128);
-          else if (w + 1 < heads)
-            load_values(w + 1, (warp - 4) * 32);
         }
       }
     }
@@ -735,16 +733,18 @@ int launch_delta_chunk(DeltaChunkParams p, cudaStream_t st) {
   // The scan's CTAs as narrow as one wave of them allows, so that fewer warps share a scheduler.
   int groups = 2;
   while (groups < kMostGroups && static_cast<long long>(p.heads) * ((p.dv + 16 * groups - 1) / (16 * groups)) > kSms) ++groups;
-  constexpr int kPrepSmem = 3 * S::kKeyBytes + static_cast<int>(sizeof(PrepShared));
-  static_assert(2 * kPrepSmem <= 226 * 1024 && Z::smem(kMostGroups) <= 227 * 1024, "shared memory of an SM");
-  const auto prepare = delta_chunk_prepare_kernel<DK>;
-  const auto scan = groups == 2 ? delta_chunk_scan_kernel<DK, 2> : delta_chunk_scan_kernel<DK, kMostGroups>;
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(prepare), kPrepSmem)) return rc;
-  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(scan), groups == 2 ? Z::smem(2) : Z::smem(kMostGroups))) return rc;
+  const int prep_smem = 2 * S::kKeyBytes + static_cast<int>(sizeof(PrepShared)) + min(kPrepHeads, p.heads / p.k_heads) * static_cast<int>(sizeof(PrepHead));
+  constexpr int kPrepMost = 2 * S::kKeyBytes + static_cast<int>(sizeof(PrepShared)) + kPrepHeads * static_cast<int>(sizeof(PrepHead));
+  static_assert(2 * kPrepMost <= 226 * 1024 && Z::smem(kMostGroups) <= 227 * 1024, "shared memory of an SM");
+  const auto scan = groups == 2 ? delta_chunk_scan_kernel<DK, 2> : groups == 3 ? delta_chunk_scan_kernel<DK, 3> : delta_chunk_scan_kernel<DK, 4>;
+  if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(scan), Z::smem(groups))) return rc;
   for (int r0 = 0; r0 < rows; r0 += kMostChunks * kChunk) {
     p.rows = min(rows - r0, kMostChunks * kChunk);
     p.chunks = (p.rows + kChunk - 1) / kChunk;
-    prepare<<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.k_heads)), kPrepThreads, kPrepSmem, st>>>(p);
+    // one CTA an SM: 255 registers a thread against 128 (64 rows: 20.6 us against 22.6; 2048 rows, seven CTAs an SM: 192 against 181)
+    const auto prepare = p.chunks * p.k_heads <= kSms ? delta_chunk_prepare_kernel<DK, 1> : delta_chunk_prepare_kernel<DK, 2>;
+    if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(prepare), kPrepMost)) return rc;  // (once a kernel: the most it may ask for)
+    prepare<<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.k_heads)), kPrepThreads, prep_smem, st>>>(p);
     if (int rc = check_launch()) return rc;
     // (may start once the first kernel's CTAs have: it loads the state, which they do not write, and waits)
     if (launch_kernel(scan, dim3(static_cast<unsigned>(p.heads), static_cast<unsigned>((p.dv + 16 * groups - 1) / (16 * groups))), dim3(128 * groups),
