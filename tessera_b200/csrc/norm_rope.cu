@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
   constexpr bool kQuant = OUT == TSR_KV_INT8 || OUT == TSR_KV_INT4 || OUT == TSR_KV_FP8;
   constexpr int kRuns = kNormMaxDim / (32 * VEC);
   extern __shared__ float k_row[];  // quantised formats: the row's k heads
-  __shared__ float cos_s[kNormMaxDim / 2], sin_s[kNormMaxDim / 2];
+  __shared__ __align__(16) float cos_s[kNormMaxDim / 2], sin_s[kNormMaxDim / 2];
   __shared__ __align__(16) float head_s[kNormWarps][kNormMaxDim];
   __shared__ float most_s[2][kNormWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = p.head_dim, pairs = p.rope_dim / 2;
@@ -103,14 +103,14 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
   const int h1 = keys ? p.kv_heads : min(p.heads, h0 + p.heads_per_cta);
   const float* src = (keys ? p.k : p.q) + row * (keys ? p.kv_heads : p.heads) * dim;
   const float* weight = keys ? p.k_w : p.q_w;
-  float x[kRuns][VEC];
+  float next[kRuns][VEC];  // a head ahead
   auto load = [&](int h) {
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
       const int e = (i * 32 + lane) * VEC;
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) x[i][c] = 0.0f;
-      if (h < h1 && e < dim) load_floats(x[i], src + static_cast<size_t>(h) * dim + e);
+      for (int c = 0; c < VEC; ++c) next[i][c] = 0.0f;
+      if (h < h1 && e < dim) load_floats(next[i], src + static_cast<size_t>(h) * dim + e);
     }
   };
   load(h0 + warp);
@@ -127,14 +127,14 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
     const int e = (i * 32 + lane) * VEC;
     if (e < dim) load_floats(w[i], weight + e);
   }
-  __syncthreads();
-  float most = 0.0f;
-  for (int h = h0 + warp; h < h1; h += kNormWarps) {
+  float most = 0.0f, x[kRuns][VEC];
+  auto normalise = [&](int h) {  // x of head h; what is rotated to shared memory too
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kRuns; ++i)
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) sum = fmaf(x[i][c], x[i][c], sum);
+      for (int c = 0; c < VEC; ++c) x[i][c] = next[i][c], sum = fmaf(x[i][c], x[i][c], sum);
+    load(h + kNormWarps);  // (in place: another head)
     const float gain = 1.0f / sqrtf(warp_sum(sum) / static_cast<float>(dim) + p.eps);
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
@@ -142,21 +142,32 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
       if (e >= dim) continue;
 #pragma unroll
       for (int c = 0; c < VEC; ++c) x[i][c] = x[i][c] * gain * w[i][c];
-      store_floats(&head_s[warp][e], x[i]);
+      if (e < p.rope_dim) store_floats(&head_s[warp][e], x[i]);
     }
     __syncwarp();
+  };
+  normalise(h0 + warp);
+  __syncthreads();  // the angles, formed meanwhile
+  for (int h = h0 + warp; h < h1; h += kNormWarps) {
 #pragma unroll
     for (int i = 0; i < kRuns; ++i) {
       const int e = (i * 32 + lane) * VEC;
       if (e >= dim) continue;
+      if (e < p.rope_dim) {  // (VEC divides the pairs)
+        const bool first = e < pairs;
+        const int d = first ? e : e - pairs;
+        float other[VEC], cosine[VEC], sine[VEC];
+        load_floats(other, &head_s[warp][first ? e + pairs : d]);
+        load_floats(cosine, &cos_s[d]), load_floats(sine, &sin_s[d]);
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) {
-        const int d = e + c;
-        if (d < pairs) x[i][c] = __fsub_rn(__fmul_rn(x[i][c], cos_s[d]), __fmul_rn(head_s[warp][d + pairs], sin_s[d]));
-        else if (d < p.rope_dim)
-          x[i][c] = __fadd_rn(__fmul_rn(head_s[warp][d - pairs], sin_s[d - pairs]), __fmul_rn(x[i][c], cos_s[d - pairs]));
-        if (kQuant) most = fmaxf(most, fabsf(x[i][c]));
+        for (int c = 0; c < VEC; ++c) {
+          const float turned = __fmul_rn(other[c], sine[c]);
+          x[i][c] = __fadd_rn(__fmul_rn(x[i][c], cosine[c]), first ? -turned : turned);
+        }
       }
+      if constexpr (kQuant)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) most = fmaxf(most, fabsf(x[i][c]));
       if (!keys) {
         store_floats(p.q_out + (row * p.heads + h) * dim + e, x[i]);
       } else {
@@ -167,7 +178,7 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
       }
     }
     __syncwarp();
-    load(h + kNormWarps);
+    if (h + kNormWarps < h1) normalise(h + kNormWarps);
   }
   if (!keys || OUT == kToFloat) return;
   // the row of v
@@ -268,7 +279,7 @@ int qk_norm_rope(const float* q, const float* k, const float* q_w, const float* 
     if ((qo.meets(r) && !(r.at == q && q_out == q)) || (ko.meets(r) && !(r.at == k && k_out == k))) return kInvalidArgument;
   if (dry) return kOk;
   p.k_out = k_out;
-  const bool vec = head_dim % 4 == 0 && wide(q) && wide(k) && wide(q_w) && wide(k_w) && wide(q_out) && wide(k_out);
+  const bool vec = head_dim % 4 == 0 && rope_dim % 8 == 0 && wide(q) && wide(k) && wide(q_w) && wide(k_w) && wide(q_out) && wide(k_out);
   return launch_norm_rope<kToFloat>(p, rows, vec, st);
 }
 
@@ -307,7 +318,7 @@ int qk_norm_rope_append(int kv_format, const float* q, const float* k, const flo
     for (int j = 0; j < i; ++j)
       if (out[i].meets(out[j])) return kInvalidArgument;
   }
-  const bool vec = head_dim % 4 == 0 && wide(q) && wide(k) && wide(v) && wide(q_w) && wide(k_w) && wide(q_out) &&
+  const bool vec = head_dim % 4 == 0 && rope_dim % 8 == 0 && wide(q) && wide(k) && wide(v) && wide(q_w) && wide(k_w) && wide(q_out) &&
                    (quant || (wide(p.k_cache) && wide(p.v_cache)));
   if (dry) return kOk;
   switch (kv_format) {
