@@ -967,7 +967,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
         tc_after();
         if (ok) outputs(t, h);
       }
-      next_scores(t + 2);  // over this tile's weights, behind the products that read them
+      if (t + 2 < tiles) wait(&sh.o_full, S::kHalves * (t + 1) - 1);  // the next scores go over this tile's weights
+      next_scores(t + 2);
     }
     if (!ok) {  // products may be under way still: not while tensor memory is given back
       tc_commit(&sh.drained);
