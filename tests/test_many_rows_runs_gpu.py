@@ -295,3 +295,24 @@ def test_tree_over_scales_far_apart(backend, kind, spread):
 def test_logprob_of_small_vocabularies(backend, vocab):
     x = np.random.default_rng(vocab).standard_normal((3, vocab)).astype(np.float32)
     check_logprob(backend, x, np.array([0, vocab - 1, vocab], np.uint32), min(32, vocab))
+
+
+@pytest.mark.parametrize("what", ["random", "rising", "falling", "equal", "steps", "late", "lowest"])
+@pytest.mark.parametrize("top_k", [1, 32])
+def test_logprob_of_many_rows_of_many_tiles(backend, what, top_k):
+    """More rows than the machine has room for two CTAs of: a CTA walks over the whole row, the list fills on the way."""
+    rows, vocab = 150, 50001 if what == "steps" else 50000
+    g = np.random.default_rng(80)
+    x = g.standard_normal((rows, vocab)).astype(np.float32)
+    if what in ("rising", "falling"):
+        x = np.sort(x, 1)[:, ::1 if what == "rising" else -1].copy()
+    elif what == "equal":
+        x[:] = 0.25
+    elif what == "steps":
+        x = np.round(x)
+    elif what == "late":  # a flood after a long calm
+        x[:, 30000:] += 20.0
+        x[::2, 45000:] += np.linspace(0, 5, vocab - 45000, dtype=np.float32)
+    elif what == "lowest":
+        x[:, 9000:40000] = np.finfo(np.float32).min
+    check_logprob(backend, x, g.integers(0, vocab, rows).astype(np.uint32), top_k)
