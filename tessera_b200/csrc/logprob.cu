@@ -12,6 +12,12 @@
 // over its inverted index, so that no two are equal and the lowest index wins among equal logits.  The first threshold is a
 // bound from the threads' maxima (enough threads are above it), and a tile that floods the list all the same (ascending or
 // equal logits) finds its own threshold by bisection over the entries.  The CTAs meet through distributed shared memory.
+//
+// Measured: 1 row of 151936, 20 tokens 13.2 us (16 CTAs: a launch, two cuts of a list and the meeting of the CTAs); 16 rows, 8
+// tokens 16.4 us; 256 rows, 20 tokens 55 us.  Of the last 35 us go without any tokens asked for (15 instructions a logit, half
+// of the issue slots taken), the rest into the lists.  256 threads a CTA, twice as many of them, took 57 us; a look at the
+// list every fourth tile instead of every one 54 us, but 18 for the 16 rows; a tile's second reading from memory instead of registers
+// 117 us.
 #include <cuda_runtime.h>
 
 #include <atomic>
