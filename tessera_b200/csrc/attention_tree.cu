@@ -132,11 +132,11 @@ __global__ void __launch_bounds__(kTreeWarps * 32) attention_tree_rows_kernel(co
 //   warps 8-10  keys and values: global memory -> binary16 in the operands' layout
 //   warp 11     one thread issues the MMAs: a tile's outputs, then the scores of the tile after next over its weights
 // Measured, 24 heads over 4 of 256 unless said: FP8, 16 rows behind 512 20.5 us; fp16, 61 rows behind 4000, 16 heads over 2 of 128
-// 28.5 us; fp32, 8 rows behind 4096 58 us; FP8, 64 rows behind 32768 152 us (the MMAs' operations alone 31 us).
+// 28.5 us; fp32, 8 rows behind 4096 39 us; FP8, 64 rows behind 32768 152 us (the MMAs' operations alone 31 us).
 // A kernel key by key (as attention_tree_rows_kernel) took 61, 391, 981 and 10389 us.  What bounds: one tile costs 13 us
 // (tensor memory, paths, two terms of the queries, the first scores) and the second launch, which joins the chunks, 3 to 4; a
 // long row of tiles the issue of its MMAs, 48 a tile of about 70 clocks whatever their width (tensor pipe 42 % busy); the fp32 cache
-// its loaders, which scale and split every row.  Tiles of 64 keys, since two tiles' weights lie over their scores and columns
+// its loaders, which scale and split every row (9 us a tile; 12 with stores of a row at a time, 16 of them to the same banks).  Tiles of 64 keys, since two tiles' weights lie over their scores and columns
 // of tensor memory are short.  Bytes by bulk copies of a key each 295 us for the long case, by tiled copies 152.
 constexpr int kSoftThreads = 256, kLoadThreads = 96, kTcThreads = kSoftThreads + kLoadThreads + 32;
 constexpr int kTcRows = 128, kTcKeys = 64;
@@ -161,8 +161,8 @@ struct TcShape {
   static constexpr bool kRaw = KV != kKvF32 && KV != kKvF16;          // raw bytes pass through shared memory
   static constexpr int kBox = kRowBytes < 128 ? kRowBytes : 128;      // bytes of a key in a box of raw bytes; 128: swizzled
   static constexpr int kRawBytes = kRaw ? kTcKeys * kRowBytes : 0;
-  static constexpr int kRun = 4, kRuns = 5, kRunsOfTile = (kTcKeys / (kLoadThreads / 32) + kRun) / kRun;  // fp32: rows of a warp under way
-  static constexpr int kRing = KV == kKvF32 ? kLoadThreads / 32 * kRuns * kRun * kRowBytes : 0;
+  static constexpr int kRuns = 768 / D, kPitch = kRowBytes + 16;      // fp32: runs of eight rows of a warp under way
+  static constexpr int kRing = KV == kKvF32 ? kLoadThreads / 32 * kRuns * 8 * kPitch : 0;
   static constexpr int kHalves = D / 128;
   static constexpr uint32_t kGroupBytes = D / 8 * 128;                // eight keys
   static constexpr int kSmem = 1024 + 2 * kBufs * kTileBytes + 4 * kRawBytes + kRing;
@@ -470,80 +470,87 @@ struct TcLoader {
       }
     }
   }
-  // fp32 rows pass through a warp's own ring, a run of four at a time and four runs ahead; a lane reads what it asked for.
-  // Run s of a warp: tile s / (2 kRunsOfTile), its keys first, then its values.
+  // fp32 rows pass through a warp's own ring, eight keys (a group of the operand's layout) a run.  Of a tile's eight runs of keys
+  // warp w takes w, w + 3, ..., of its eight runs of values (w + 2) % 3 and so on: five, six and five.
+  __device__ __forceinline__ int runs_of_keys(int warp) const { return warp == 2 ? 2 : 3; }
+  __device__ __forceinline__ int runs_of_tile(int warp) const { return warp == 1 ? 6 : 5; }
+  __device__ __forceinline__ unsigned char* run_at(int s, unsigned char* ring, int warp) const {
+    return ring + (warp * S::kRuns + s % S::kRuns) * 8 * S::kPitch;
+  }
   __device__ __forceinline__ void ask_rows(int s, unsigned char* ring, int tid) const {
-    const int lane = tid & 31, warp = tid >> 5;
-    if (s < tiles * 2 * S::kRunsOfTile) {
-      const int t = s / (2 * S::kRunsOfTile), x = s - t * 2 * S::kRunsOfTile;
-      const bool values = x >= S::kRunsOfTile;
-      const int k0 = (values ? x - S::kRunsOfTile : x) * S::kRun * (kLoadThreads / 32) + warp;
-      unsigned char* dst = ring + ((warp * S::kRuns + s % S::kRuns) * S::kRun) * S::kRowBytes + lane * 16;
+    static_assert(kLoadThreads == 96, "three warps");
+    const int lane = tid & 31, warp = tid >> 5, of_tile = runs_of_tile(warp), of_keys = runs_of_keys(warp);
+    const int t = s / of_tile, x = s - t * of_tile;
+    if (t < tiles) {
+      const bool values = x >= of_keys;
+      const int group = values ? (warp + 2) % 3 + 3 * (x - of_keys) : warp + 3 * x;
+      unsigned char* dst = run_at(s, ring, warp) + lane * 16;
 #pragma unroll
-      for (int u = 0; u < S::kRun; ++u) {
-        const int key = k0 + u * (kLoadThreads / 32), j = min(c0 + t * kTcKeys + key, c1 - 1);
+      for (int u = 0; u < 8; ++u) {
+        const int j = min(c0 + t * kTcKeys + group * 8 + u, c1 - 1);
         const unsigned char* src = base(values) + j * pitch() + lane * 16;
-        if (key < kTcKeys) {
 #pragma unroll
-          for (int i = 0; i < D / 128; ++i)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + u * S::kRowBytes + i * 512), "l"(src + i * 512) : "memory");
-        }
+        for (int i = 0; i < D / 128; ++i)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst) + u * S::kPitch + i * 512), "l"(src + i * 512) : "memory");
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  // Each row scaled by a power of two to [2^13, 2^14), two terms.
+  // Each row scaled by a power of two to [2^13, 2^14), two terms.  Row by row for its largest element; then a lane has a row,
+  // eight elements at a time, so that the ring's rows (16 bytes apart in their banks) and the operand's are free of conflicts.
   __device__ __forceinline__ void split_rows(bool values, int t, unsigned char* ring, unsigned char* dst, int tid) const {
-    constexpr int kLoadWarps = kLoadThreads / 32, kPer = D / 128;
-    const int lane = tid & 31, warp = tid >> 5;
+    const int lane = tid & 31, warp = tid >> 5, of_keys = runs_of_keys(warp), key = lane & 7;
+    const int runs = values ? runs_of_tile(warp) - of_keys : of_keys;
     int high = kNoExponent, low = -kNoExponent;
 #pragma unroll 1
-    for (int b = 0; b < S::kRunsOfTile; ++b) {
-      const int s = (2 * t + (values ? 1 : 0)) * S::kRunsOfTile + b;
+    for (int b = 0; b < runs; ++b) {
+      const int s = t * runs_of_tile(warp) + (values ? of_keys : 0) + b, group = (values ? (warp + 2) % 3 : warp) + 3 * b;
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kRuns - 1) : "memory");
-      const unsigned char* src = ring + ((warp * S::kRuns + s % S::kRuns) * S::kRun) * S::kRowBytes + lane * 16;
-      float4 x[S::kRun][kPer];
+      __syncwarp();
+      const unsigned char* const rows = run_at(s, ring, warp);
+      uint32_t most[8];
 #pragma unroll
-      for (int u = 0; u < S::kRun; ++u)
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) x[u][i] = *reinterpret_cast<const float4*>(src + u * S::kRowBytes + i * 512);
-      uint32_t most[S::kRun];
-#pragma unroll
-      for (int u = 0; u < S::kRun; ++u) {
-        const int key = (b * S::kRun + u) * kLoadWarps + warp, j = min(c0 + t * kTcKeys + key, c1 - 1);
-        const bool zero = key >= kTcKeys || (j >= p.t.n && unseen(j));
+      for (int u = 0; u < 8; ++u) {
         most[u] = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if (zero) x[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          most[u] = max(max(most[u], max(__float_as_uint(x[u][i].x) & 0x7FFFFFFFu, __float_as_uint(x[u][i].y) & 0x7FFFFFFFu)),
-                        max(__float_as_uint(x[u][i].z) & 0x7FFFFFFFu, __float_as_uint(x[u][i].w) & 0x7FFFFFFFu));
+        for (int i = 0; i < D / 128; ++i) {
+          const uint4 y = *reinterpret_cast<const uint4*>(rows + u * S::kPitch + i * 512 + lane * 16);
+          most[u] = max(max(most[u], max(y.x & 0x7FFFFFFFu, y.y & 0x7FFFFFFFu)), max(y.z & 0x7FFFFFFFu, y.w & 0x7FFFFFFFu));
         }
       }
+      uint32_t mine = 0;
 #pragma unroll
-      for (int u = 0; u < S::kRun; ++u) most[u] = __reduce_max_sync(0xFFFFFFFFu, most[u]);
-#pragma unroll
-      for (int u = 0; u < S::kRun; ++u) {
-        const int key = (b * S::kRun + u) * kLoadWarps + warp;
-        const int e = most[u] == 0 ? 0 : max(-110, min(114, static_cast<int>(most[u] >> 23) - 127 - 13));
-        const float up = power_of_two(-e);
-        if (most[u] != 0) high = max(high, e), low = min(low, e);
-        if (key < kTcKeys) {
-          if (lane == 0) sh.scale[t % kScaleBufs][values ? 1 : 0][key] = power_of_two(e);
-          unsigned char* at = dst + (key / 8) * S::kGroupBytes + (key % 8) * 16 + lane / 2 * 128 + (lane & 1) * 8;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            uint2 hi, lo;
-            tree_split(x[u][i].x * up, x[u][i].y * up, hi.x, lo.x);
-            tree_split(x[u][i].z * up, x[u][i].w * up, hi.y, lo.y);
-            *reinterpret_cast<uint2*>(at + i * 2048) = hi;
-            *reinterpret_cast<uint2*>(at + i * 2048 + S::kTermBytes) = lo;
-          }
-        }
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t all = __reduce_max_sync(0xFFFFFFFFu, most[u]);
+        mine = key == u ? all : mine;
       }
+      const int j = min(c0 + t * kTcKeys + group * 8 + key, c1 - 1);
+      const bool zero = j >= p.t.n && unseen(j);
+      if (zero) mine = 0;
+      const int e = mine == 0 ? 0 : max(-110, min(114, static_cast<int>(mine >> 23) - 127 - 13));
+      const float up = power_of_two(-e);
+      if (mine != 0) high = max(high, e), low = min(low, e);
+      if (lane < 8) sh.scale[t % kScaleBufs][values ? 1 : 0][group * 8 + key] = power_of_two(e);
+#pragma unroll 4
+      for (int it = 0; it < D / 32; ++it) {
+        const int c = it * 4 + (lane >> 3);
+        float4 x = *reinterpret_cast<const float4*>(rows + key * S::kPitch + c * 32), y = *reinterpret_cast<const float4*>(rows + key * S::kPitch + c * 32 + 16);
+        if (zero) x = y = make_float4(0.f, 0.f, 0.f, 0.f);
+        uint4 hi, lo;
+        tree_split(x.x * up, x.y * up, hi.x, lo.x);
+        tree_split(x.z * up, x.w * up, hi.y, lo.y);
+        tree_split(y.x * up, y.y * up, hi.z, lo.z);
+        tree_split(y.z * up, y.w * up, hi.w, lo.w);
+        unsigned char* const at = dst + group * S::kGroupBytes + key * 16 + c * 128;
+        *reinterpret_cast<uint4*>(at) = hi;
+        *reinterpret_cast<uint4*>(at + S::kTermBytes) = lo;
+      }
+      __syncwarp();  // the run's place is free
       ask_rows(s + S::kRuns, ring, tid);
     }
-    if (values && lane == 0) sh.range[t % kScaleBufs][warp][0] = high, sh.range[t % kScaleBufs][warp][1] = low;
+    if (!values) return;
+    high = __reduce_max_sync(0xFFFFFFFFu, high), low = __reduce_min_sync(0xFFFFFFFFu, low);
+    if (lane == 0) sh.range[t % kScaleBufs][warp][0] = high, sh.range[t % kScaleBufs][warp][1] = low;
   }
   // a quantised tile's scales: asked for a tile ahead, put where the weights are formed
   __device__ __forceinline__ void next_scales(int t, int tid, float& k, float& v) const {
@@ -1073,7 +1080,9 @@ int launch_tree(const TreeParams& t, uint64_t head_dim, cudaStream_t st) {
   p.first_key = t.window != 0 && t.window < t.n ? t.n - t.window : 0;
   const long keys = static_cast<long>(t.n) + t.m - p.first_key, tiles = (keys + kTcKeys - 1) / kTcKeys;
   const long units = static_cast<long>(t.kv_heads) * p.row_tiles;
-  // Chunks of the key range: whole waves of one CTA a SM, a CTA's start counted as four tiles.
+  // Chunks of the key range: whole waves of one CTA a SM, a CTA's start counted as four tiles; a tile of the fp32 cache costs its
+  // loaders three of the others' (65 tiles of 8 rows, 4 kv heads: 33 chunks of two tiles 39 us, 22 of three 49, 17 of four 58).
+  const double tile_cost = KV == kKvF32 ? (head_dim == 256 ? 3.0 : 1.5) : 1.0;
   static const int sms = [] {
     int dev = 0, v = 0;
     cudaGetDevice(&dev);
@@ -1086,7 +1095,7 @@ int launch_tree(const TreeParams& t, uint64_t head_dim, cudaStream_t st) {
     const long per = (tiles + s - 1) / s;
     if ((tiles + per - 1) / per != s) continue;
     const double waves = static_cast<double>((units * s + sms - 1) / sms);
-    const double cost = waves * (per + 4.0) + (s > 1 ? 2.0 + 0.1 * s : 0.0);
+    const double cost = waves * (per * tile_cost + 4.0) + (s > 1 ? 2.0 + 0.1 * s : 0.0);
     if (s == 1 || cost < best) best = cost, best_splits = s;
   }
   p.splits = static_cast<int>(best_splits);
