@@ -591,7 +591,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
 
   if (tid < kTreeWords) sh.used[tid] = 0;
   if (tid < kTcRows) sh.bad[tid] = 0;
-  if (tid < p.t.m) sh.parents[tid] = p.t.parents[tid];
   if (tid == 0) {
     sh.any_bad = 0;
     for (int b = 0; b < 2; ++b) {
@@ -604,6 +603,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     mbar_fence_init();
   }
   if (warp == kTcThreads / 32 - 1) tc_alloc(&sh.tmem);
+  // (so far this kernel's start overlaps the end of the one before it)
+  pdl_trigger();
+  pdl_wait();
+  if (tid < p.t.m) sh.parents[tid] = p.t.parents[tid];
   // Queries, to begin with as they are, in the operands' buffers: 16-byte piece c of a row at c ^ (row & 7).
   if (warp < kSoftThreads / 32) {
     constexpr int kRowsOf = kTcRows / (kSoftThreads / 32);
@@ -1002,6 +1005,7 @@ template <int D>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 attention_tree_merge_kernel(const float* __restrict__ pacc, const float* __restrict__ pmax, const float* __restrict__ psum,
                             float* __restrict__ out, int splits, int total) {
+  pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const size_t row = static_cast<size_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
@@ -1051,7 +1055,11 @@ int launch_tree_tc(TcParams p, cudaStream_t st) {
       if (int rc = encode_tensor_map(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, i ? p.t.v : p.t.k, dims, &stride, box, S::kBox == 128)) return rc;
   }
   const dim3 grid(static_cast<unsigned>(p.t.kv_heads * p.row_tiles), static_cast<unsigned>(p.splits));
-  kernel<<<grid, kTcThreads, S::kSmem, st>>>(maps[0], maps[1], p);
+  const bool pdl = pdl_allowed(st, nullptr, 0, p.t.out, static_cast<size_t>(p.t.m) * p.t.heads * D * 4);
+  if (launch_kernel(kernel, grid, dim3(kTcThreads), S::kSmem, st, pdl, maps[0], maps[1], p) != cudaSuccess) {
+    cudaGetLastError();
+    return kDeviceError;
+  }
   if (int rc = check_launch(); rc != kOk || p.pacc == nullptr) return rc;
   const int total = p.t.m * p.t.heads;
   // (its launch overlaps the end of the chunks' kernel, which it waits for before it reads or writes anything)

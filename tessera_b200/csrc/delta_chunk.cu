@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(kPrepThreads, PER_SM) delta_chunk_prepare_kern
   unsigned char *const op_s = prep_smem, *const w_s = prep_smem + S::kKeyBytes;
   PrepShared& sh = *reinterpret_cast<PrepShared*>(prep_smem + 2 * S::kKeyBytes);
   PrepHead* const hd = reinterpret_cast<PrepHead*>(prep_smem + 2 * S::kKeyBytes + sizeof(PrepShared));  // as many as there are, at most kPrepHeads
-  pdl_trigger();  // (once every CTA has started, the scan's may)
+  pdl_wait();     // (this kernel's start overlaps the end of the one before it)
+  pdl_trigger();  // once every CTA is here, the scan's may start: not earlier, since they read the state ahead of their wait
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
   const int chunk = blockIdx.x, kh = blockIdx.y, t0 = chunk * kChunk, rows = min(kChunk, p.rows - t0), factor = p.heads / p.k_heads;
   float alpha = 1.0f, beta = 0.0f;  // of row `lane` and the value head that the warp solves
@@ -538,11 +539,11 @@ __global__ void __launch_bounds__(GROUPS * 128, 1) delta_chunk_scan_kernel(const
   const size_t o_step = static_cast<size_t>(p.heads) * p.dv, o_at = static_cast<size_t>(h) * p.dv + col + g;
   float s[kTiles][4];  // S^T: columns g, g + 8 of the state, rows 8 n + 2 t + {0, 1} of this half
   const size_t state = (static_cast<size_t>(h) * DK + half * (DK / 2)) * p.dv + col + g;
-  if (carries && active) {  // (the kernel before this one does not write it)
+  if (carries && active) {  // (the kernel before this one does not write it, and has waited for those that may have)
 #pragma unroll
     for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[n][c] = p.s[state + static_cast<size_t>(8 * n + 2 * t + (c & 1)) * p.dv + 8 * (c >> 1)];
+      for (int c = 0; c < 4; ++c) s[n][c] = __ldcg(p.s + state + static_cast<size_t>(8 * n + 2 * t + (c & 1)) * p.dv + 8 * (c >> 1));
   }
   const bool stages = warp == 2 && lane == 0;  // (of a warp that does not carry)
   if (stages) {
@@ -551,6 +552,7 @@ __global__ void __launch_bounds__(GROUPS * 128, 1) delta_chunk_scan_kernel(const
   }
   __syncthreads();
   pdl_wait();
+  pdl_trigger();
   if (stages) stage(0);
   bool ok = true;
   // matrices of an ldmatrix: rows 0-7 / 8-15 (lane / 16), first / second eight elements of a step (lane / 8 % 2)
@@ -752,7 +754,14 @@ int launch_delta_chunk(DeltaChunkParams p, cudaStream_t st) {
     // one CTA an SM: 255 registers a thread against 128 (64 rows: 20.6 us against 22.6; 2048 rows, seven CTAs an SM: 192 against 181)
     const auto prepare = p.chunks * p.k_heads <= kSms ? delta_chunk_prepare_kernel<DK, 1> : delta_chunk_prepare_kernel<DK, 2>;
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(prepare), kPrepMost)) return rc;  // (once a kernel: the most it may ask for)
-    prepare<<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.k_heads)), kPrepThreads, prep_smem, st>>>(p);
+    const void* const out[2] = {p.o, p.s_out};
+    const size_t out_bytes[2] = {static_cast<size_t>(p.rows) * p.heads * p.dv * 4, static_cast<size_t>(p.heads) * DK * p.dv * 4};
+    const bool pdl = pdl_allowed_ranges(st, nullptr, nullptr, 0, out, out_bytes, 2);
+    if (launch_kernel(prepare, dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.k_heads)), dim3(kPrepThreads), static_cast<size_t>(prep_smem), st,
+                      pdl, p) != cudaSuccess) {
+      cudaGetLastError();
+      return kDeviceError;
+    }
     if (int rc = check_launch()) return rc;
     // (may start once the first kernel's CTAs have: it loads the state, which they do not write, and waits)
     if (launch_kernel(scan, dim3(static_cast<unsigned>(p.heads), static_cast<unsigned>((p.dv + 16 * groups - 1) / (16 * groups))), dim3(128 * groups),

@@ -168,8 +168,10 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
       }
     }
   };
-  load(begin);
   if (tid == 0) sh.count = 0;
+  pdl_trigger();
+  pdl_wait();  // (this kernel's start overlaps the end of the one before it)
+  load(begin);
   float given = -INFINITY;  // the target's logit
   if (rank == 0 && tid == 0) {
     const uint32_t target = targets[row];
@@ -380,7 +382,8 @@ int launch_logprob(unsigned ctas, uint64_t rows, const float* logits, const uint
       }
     }
   }
-  const cudaError_t e = launch_kernel_cluster(kernel, dim3(ctas, static_cast<unsigned>(rows)), dim3(THREADS), sizeof(LogprobShared), st, false, ctas, logits, targets, logprob,
+  const bool pdl = pdl_allowed(st, nullptr, 0, logprob, rows * 4);
+  const cudaError_t e = launch_kernel_cluster(kernel, dim3(ctas, static_cast<unsigned>(rows)), dim3(THREADS), sizeof(LogprobShared), st, pdl, ctas, logits, targets, logprob,
                                               entropy, top_ids, top_logprobs, static_cast<uint32_t>(vocab), static_cast<int>(top_k), row_base);
   if (e != cudaSuccess) {
     cudaGetLastError();

@@ -119,10 +119,14 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
       if (h < h1 && e < dim) load_floats(next[i], src + static_cast<size_t>(h) * dim + e);
     }
   };
+  // (this kernel's start overlaps the end of the one before it, which may write anything that is read from here on)
+  pdl_trigger();
+  const double freq = tid < pairs ? exp2(p.log2_theta * (-2.0 * tid / p.rope_dim)) : 0.0;
+  pdl_wait();
   load(h0 + warp);
   if (tid < pairs) {
     const unsigned long long at = p.pos[row * 3 + (tid < p.sec_t ? 0 : tid < p.sec_t + p.sec_h ? 1 : 2)];
-    const double angle = static_cast<double>(at) * exp2(p.log2_theta * (-2.0 * tid / p.rope_dim));
+    const double angle = static_cast<double>(at) * freq;
     double s, c;
     sincos(angle, &s, &c);
     cos_s[tid] = static_cast<float>(c), sin_s[tid] = static_cast<float>(s);
@@ -243,8 +247,11 @@ int launch_norm_rope(NormRopeParams& p, uint64_t rows, bool vec, cudaStream_t st
   p.heads_per_cta = (p.heads + parts - 1) / parts;
   const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(1 + parts));
   const size_t smem = kQuant ? static_cast<size_t>(p.kv_heads) * p.head_dim * 4 : 0;
-  if (vec) qk_norm_rope_kernel<OUT, 4><<<grid, kNormThreads, smem, st>>>(p);
-  else qk_norm_rope_kernel<OUT, 1><<<grid, kNormThreads, smem, st>>>(p);
+  const bool pdl = pdl_allowed(st, nullptr, 0, p.q_out, rows * p.heads * p.head_dim * 4);
+  if (launch_kernel(vec ? qk_norm_rope_kernel<OUT, 4> : qk_norm_rope_kernel<OUT, 1>, grid, dim3(kNormThreads), smem, st, pdl, p) != cudaSuccess) {
+    cudaGetLastError();
+    return kDeviceError;
+  }
   return check_launch();
 }
 
