@@ -603,8 +603,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
     mbar_fence_init();
   }
   if (warp == kTcThreads / 32 - 1) tc_alloc(&sh.tmem);
-  // (so far this kernel's start overlaps the end of the one before it)
-  pdl_trigger();
+  // So far this kernel's start overlaps the end of the one before it.  (It lets no other start under its own end: the registers are
+  // taken, and CTAs that wait elsewhere cost the long case 5 of 151 us.)
   pdl_wait();
   if (tid < p.t.m) sh.parents[tid] = p.t.parents[tid];
   // Queries, to begin with as they are, in the operands' buffers: 16-byte piece c of a row at c ^ (row & 7).
