@@ -149,7 +149,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
   return max(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
 }
 
-// grid: (chunks, key heads), 8 warps.  Up to four value heads at a time: the substitution is a warp's, everything else is spread
+// grid: (chunks, key heads, parts of a key head's value heads), 8 warps.  Up to four value heads at a time: the substitution is a warp's, everything else is spread
 // over all warps.
 constexpr int kPrepThreads = 256, kPrepWarps = kPrepThreads / 32, kPrepHeads = 4, kPitch = kChunk + 4;
 struct PrepHead {
@@ -173,14 +173,15 @@ __global__ void __launch_bounds__(kPrepThreads, PER_SM) delta_chunk_prepare_kern
   pdl_wait();     // (this kernel's start overlaps the end of the one before it)
   pdl_trigger();  // once every CTA is here, the scan's may start: not earlier, since they read the state ahead of their wait
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int chunk = blockIdx.x, kh = blockIdx.y, t0 = chunk * kChunk, rows = min(kChunk, p.rows - t0), factor = p.heads / p.k_heads;
+  const int chunk = blockIdx.x, kh = blockIdx.y, t0 = chunk * kChunk, rows = min(kChunk, p.rows - t0);
+  const int factor = p.heads / p.k_heads, per = (factor + gridDim.z - 1) / gridDim.z, f_begin = blockIdx.z * per, f_end = min(factor, f_begin + per);
   float alpha = 1.0f, beta = 0.0f;  // of row `lane` and the value head that the warp solves
   auto load_gates = [&](int f) {
-    if (warp >= kPrepHeads || f >= factor || lane >= rows) return alpha = 1.0f, beta = 0.0f, void();
+    if (warp >= kPrepHeads || f >= f_end || lane >= rows) return alpha = 1.0f, beta = 0.0f, void();
     const size_t at = static_cast<size_t>(t0 + lane) * p.heads + kh + f * p.k_heads;
     alpha = p.alpha[at], beta = p.beta[at];
   };
-  load_gates(warp);
+  load_gates(f_begin + warp);
   // eight lanes a row
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(kPrepThreads, PER_SM) delta_chunk_prepare_kern
   const size_t step_v = static_cast<size_t>(p.heads) * p.dv;
   fence_async();
   __syncthreads();
-  if (tid == 0) bulk_store(p.keys + (static_cast<size_t>(kh) * p.chunks + chunk) * 2 * S::kKeyBytes, op_s, 2 * S::kKeyBytes);
+  if (tid == 0 && blockIdx.z == 0) bulk_store(p.keys + (static_cast<size_t>(kh) * p.chunks + chunk) * 2 * S::kKeyBytes, op_s, 2 * S::kKeyBytes);
   {  // the Gram matrices: 16 rows by 16 columns a warp; what lies above the diagonal is not used
     const int which = warp >> 2, m = warp >> 1 & 1, n = warp & 1;
     if (n <= m) {
@@ -251,8 +252,8 @@ __global__ void __launch_bounds__(kPrepThreads, PER_SM) delta_chunk_prepare_kern
         }
     }
   }
-  for (int f0 = 0; f0 < factor; f0 += kPrepHeads) {
-    const int heads = min(kPrepHeads, factor - f0);
+  for (int f0 = f_begin; f0 < f_end; f0 += kPrepHeads) {
+    const int heads = min(kPrepHeads, f_end - f0);
     Factors* const fac = p.factors + static_cast<size_t>(kh + f0 * p.k_heads) * p.chunks + chunk;
     const size_t fac_step = static_cast<size_t>(p.k_heads) * p.chunks;
     unsigned char* const mats = p.mats + (static_cast<size_t>(kh + f0 * p.k_heads) * p.chunks + chunk) * (S::kKeyBytes + S::kMatBytes);
@@ -743,7 +744,6 @@ int launch_delta_chunk(DeltaChunkParams p, cudaStream_t st) {
   // 2.0 us, of 48 2.9 us).
   int groups = 2;
   while (groups < kMostGroups && static_cast<long long>(p.heads) * ((p.dv + 16 * groups - 1) / (16 * groups)) > kSms) ++groups;
-  const int prep_smem = 2 * S::kKeyBytes + static_cast<int>(sizeof(PrepShared)) + min(kPrepHeads, p.heads / p.k_heads) * static_cast<int>(sizeof(PrepHead));
   constexpr int kPrepMost = 2 * S::kKeyBytes + static_cast<int>(sizeof(PrepShared)) + kPrepHeads * static_cast<int>(sizeof(PrepHead));
   static_assert(2 * kPrepMost <= 226 * 1024 && Z::smem(kMostGroups) <= 227 * 1024, "shared memory of an SM");
   const auto scan = groups == 2 ? delta_chunk_scan_kernel<DK, 2> : groups == 3 ? delta_chunk_scan_kernel<DK, 3> : delta_chunk_scan_kernel<DK, 4>;
@@ -751,13 +751,16 @@ int launch_delta_chunk(DeltaChunkParams p, cudaStream_t st) {
   for (int r0 = 0; r0 < rows; r0 += kMostChunks * kChunk) {
     p.rows = min(rows - r0, kMostChunks * kChunk);
     p.chunks = (p.rows + kChunk - 1) / kChunk;
+    // Where that leaves SMs without a CTA, the value heads of a key head are spread over several (33 rows: 3 of 19 us).
+    const int factor = p.heads / p.k_heads, parts = max(1, min(factor, kSms / (p.chunks * p.k_heads))), per = (factor + parts - 1) / parts;
+    const int prep_smem = 2 * S::kKeyBytes + static_cast<int>(sizeof(PrepShared)) + min(kPrepHeads, per) * static_cast<int>(sizeof(PrepHead));
     // one CTA an SM: 255 registers a thread against 128 (64 rows: 20.6 us against 22.6; 2048 rows, seven CTAs an SM: 192 against 181)
-    const auto prepare = p.chunks * p.k_heads <= kSms ? delta_chunk_prepare_kernel<DK, 1> : delta_chunk_prepare_kernel<DK, 2>;
+    const auto prepare = p.chunks * p.k_heads * ((factor + per - 1) / per) <= kSms ? delta_chunk_prepare_kernel<DK, 1> : delta_chunk_prepare_kernel<DK, 2>;
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(prepare), kPrepMost)) return rc;  // (once a kernel: the most it may ask for)
     const void* const out[2] = {p.o, p.s_out};
     const size_t out_bytes[2] = {static_cast<size_t>(p.rows) * p.heads * p.dv * 4, static_cast<size_t>(p.heads) * DK * p.dv * 4};
     const bool pdl = pdl_allowed_ranges(st, nullptr, nullptr, 0, out, out_bytes, 2);
-    if (launch_kernel(prepare, dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.k_heads)), dim3(kPrepThreads), static_cast<size_t>(prep_smem), st,
+    if (launch_kernel(prepare, dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.k_heads), static_cast<unsigned>((factor + per - 1) / per)), dim3(kPrepThreads), static_cast<size_t>(prep_smem), st,
                       pdl, p) != cudaSuccess) {
       cudaGetLastError();
       return kDeviceError;

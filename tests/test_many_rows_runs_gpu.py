@@ -316,3 +316,22 @@ def test_logprob_of_many_rows_of_many_tiles(backend, what, top_k):
     elif what == "lowest":
         x[:, 9000:40000] = np.finfo(np.float32).min
     check_logprob(backend, x, g.integers(0, vocab, rows).astype(np.uint32), top_k)
+
+
+def test_a_state_carried_from_call_to_call(backend):
+    """Prompts in pieces, the state in place, nothing waiting in between: as with a wait after every piece."""
+    stream, lib, t = torch.cuda.Stream(), capi.load_library(), Delta(8 * 45, 2, 6, 128, 64, seed=90)
+    x = {n: torch.from_numpy(getattr(t, n)).cuda() for n in ("k", "v", "q", "alpha", "beta", "s")}
+    found = []
+    for wait in (False, True):
+        s, o = x["s"].clone(), torch.zeros_like(x["v"])
+        torch.cuda.synchronize()
+        for at in range(0, t.rows, 45):
+            k, v, q, alpha, beta = (x[n][at:at + 45].data_ptr() for n in ("k", "v", "q", "alpha", "beta"))
+            assert lib.tsr_delta_chunk_heads(s.data_ptr(), k, v, q, o[at:].data_ptr(), alpha, beta, s.data_ptr(), 6, 2, 128, 64, 45, 0, 0, stream.cuda_stream) == 0
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        found.append((o.cpu().numpy(), s.cpu().numpy()))
+    assert all(np.array_equal(a, b) for a, b in zip(*found))
+    assert all(near_whole(y, r) for y, r in zip(found[0], t.want()))
