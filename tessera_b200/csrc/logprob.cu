@@ -5,7 +5,7 @@
 // a row once for every one of them.
 //
 // Bound: the logits' bytes (256 rows of 151936: 156 MB, 24 us at the measured copy rate).  A cluster of CTAs takes a row.  A
-// CTA walks over its share in tiles of 8192 logits held in registers, the next tile's loads under way, with a running maximum
+// CTA walks over its share in tiles of 6144 logits held in registers, the next tile's loads under way, with a running maximum
 // and two running sums a thread.  The likeliest tokens come out of the same registers: a logit below the threshold -- the
 // top_k-th largest so far -- costs one comparison; the few above it go to a list in shared memory, which is cut back to its
 // top_k largest by counting, for each entry, the entries above it.  An entry is its logit's bits in an order-preserving form
@@ -13,11 +13,11 @@
 // bound from the threads' maxima (enough threads are above it), and a tile that floods the list all the same (ascending or
 // equal logits) finds its own threshold by bisection over the entries.  The CTAs meet through distributed shared memory.
 //
-// Measured: 1 row of 151936, 20 tokens 13.2 us (16 CTAs: a launch, two cuts of a list and the meeting of the CTAs); 16 rows, 8
-// tokens 16.4 us; 256 rows, 20 tokens 55 us.  Of the last 35 us go without any tokens asked for (15 instructions a logit, half
-// of the issue slots taken), the rest into the lists.  256 threads a CTA, twice as many of them, took 57 us; a look at the
-// list every fourth tile instead of every one 54 us, but 18 for the 16 rows; a tile's second reading from memory instead of registers
-// 117 us.
+// Measured: 1 row of 151936, 20 tokens 10.3 us (16 CTAs: a launch, two cuts of a list and the meeting of the CTAs); 16 rows, 8
+// tokens 14.1 us; 256 rows, 20 tokens 44 us.  Twelve logits a thread are the most that the registers of two CTAs of 512
+// threads hold: 16 spilled (11.4, 15.2, 53 us), 8 take 11.0, 14.2 and 50 us.  With 16, 256 threads a CTA, twice as many of them,
+// took 57 us where 512 took 55; a look at the list every fourth tile instead of every one 54 us, but 18 for the 16 rows; a
+// tile's second reading from memory instead of registers 117 us.
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -30,7 +30,7 @@ namespace tsr {
 namespace {
 
 constexpr int kLpMost = 512;    // threads of a CTA at most
-constexpr int kLpPer = 16;      // logits of a thread at a time
+constexpr int kLpPer = 12;      // logits of a thread at a time
 constexpr int kLpList = 1024;   // entries of the list
 constexpr int kLpTop = 32;      // top_k at most, as top_k_rows
 constexpr int kLpCluster = 16;  // CTAs of a row at most
@@ -156,6 +156,15 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
   float next[kLpPer];
   auto index_of = [&](uint32_t tile, int i) { return tile + (i / VEC) * (THREADS * VEC) + tid * VEC + i % VEC; };
   auto load = [&](uint32_t tile) {
+    if (VEC == 4 && tile + kTile <= end) {  // a whole tile: no checks, no defaults
+      const float4* const from = reinterpret_cast<const float4*>(x + tile) + tid;
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        const float4 y = __ldcs(from + r * THREADS);
+        next[r * VEC] = y.x, next[r * VEC + 1 % VEC] = y.y, next[r * VEC + 2 % VEC] = y.z, next[r * VEC + 3 % VEC] = y.w;
+      }
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
       const uint32_t at = index_of(tile, r * VEC);
