@@ -131,9 +131,9 @@ __global__ void __launch_bounds__(kTreeWarps * 32) attention_tree_rows_kernel(co
 //   warps 0-7   a thread a row (tensor memory lane), warps 0-3 keys 0-31 of a tile and outputs 0-63 of a half, 4-7 the rest
 //   warps 8-10  keys and values: global memory -> binary16 in the operands' layout
 //   warp 11     one thread issues the MMAs: a tile's outputs, then the scores of the tile after next over its weights
-// Measured, 24 heads over 4 of 256 unless said: FP8, 16 rows behind 512 20.5 us; fp16, 61 rows behind 4000, 16 heads over 2 of 128
-// 28.5 us; fp32, 8 rows behind 4096 39 us; FP8, 64 rows behind 32768 152 us (the MMAs' operations alone 31 us).
-// A kernel key by key (as attention_tree_rows_kernel) took 61, 391, 981 and 10389 us.  What bounds: one tile costs 13 us
+// Measured, 24 heads over 4 of 256 unless said: FP8, 16 rows behind 512 18.1 us; fp16, 61 rows behind 4000, 16 heads over 2 of 128
+// 25 us; fp32, 8 rows behind 4096 36 us; FP8, 64 rows behind 32768 151 us (the MMAs' operations alone 31 us).
+// A kernel key by key (as attention_tree_rows_kernel) took 61, 391, 981 and 10389 us.  What bounds: one tile costs 12 us
 // (tensor memory, paths, two terms of the queries, the first scores) and the second launch, which joins the chunks, 3 to 4; a
 // long row of tiles the issue of its MMAs, 48 a tile of about 70 clocks whatever their width (tensor pipe 42 % busy); the fp32 cache
 // its loaders, which scale and split every row (9 us a tile; 12 with stores of a row at a time, 16 of them to the same banks).  Tiles of 64 keys, since two tiles' weights lie over their scores and columns

@@ -16,8 +16,8 @@
 // bits below the row's largest element, and three products of terms; in the scan small products have accumulators of their own
 // (the MMA cuts off what falls below its accumulator).
 //
-// Bound: the chain of the chunks.  48 heads over 16 key heads of 128 x 128, 512 rows: 66 us, of which 22 the first kernel (44 % of
-// its issue slots, a chain of short phases) and 48 the scan, 2.9 us a chunk; 32 heads, 2048 rows: 181 us, 61 and 128, 2.0 us a chunk
+// Bound: the chain of the chunks.  48 heads over 16 key heads of 128 x 128, 33 rows: 16 us; 512 rows: 63 us, of which 22 the first kernel (44 % of
+// its issue slots, a chain of short phases) and 48 the scan, 2.9 us a chunk; 32 heads, 2048 rows: 179 us, 61 and 128, 2.0 us a chunk
 // (tensor pipe 30 % busy, a third of the issue slots: what a warp waits for is its own last instruction).  Row by row the same
 // takes 155 us for 512 rows.  Steps: one warp for 16 whole columns, outputs by the same warp 78 and 261; outputs by warps of
 // their own, copies of 16 bytes by all threads 75 and 270 (the copies' issue held up everybody); T folded into W, half of dk a
