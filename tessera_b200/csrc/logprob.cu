@@ -1,5 +1,5 @@
 // Log probabilities of given tokens, the entropy of every row and its likeliest tokens, in one pass over the logits (id
-// "logprob_rows"): what a server answers beside a token, and what a verified tree's drafts or a scored prompt are judged by.
+// "logprob_rows"): what a server answers beside a token, and what a verified tree's drafts or a scored prompt are measured by.
 //   lse = m + log S, m = max x, S = sum e^(x - m);   logprob = x_t - lse;   entropy = log S - T / S, T = sum e^(x - m) (x - m)
 // The reference has top_k_rows for the likeliest tokens alone (src/backends/rocm/rocm_kernels.hpp:558-566), whose kernel walks
 // a row once for every one of them.

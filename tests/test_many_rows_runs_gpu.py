@@ -335,3 +335,17 @@ def test_a_state_carried_from_call_to_call(backend):
         found.append((o.cpu().numpy(), s.cpu().numpy()))
     assert all(np.array_equal(a, b) for a, b in zip(*found))
     assert all(near_whole(y, r) for y, r in zip(found[0], t.want()))
+
+
+@pytest.mark.parametrize("kind", ["f32", "fp8"])
+def test_tree_captured_before_the_first_call(backend, kind):
+    """Without a workspace the keys are not cut into chunks: the same rows but for roundings."""
+    stream, c = torch.cuda.Stream(), Typed("tree", kind, seed=91)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert c.call(stream) == 0
+    c.clear()
+    graph.replay()
+    torch.cuda.synchronize()
+    c.check(c.results())
