@@ -393,7 +393,9 @@ int launch_logprob(unsigned ctas, uint64_t rows, const float* logits, const uint
       }
     }
   }
-  const bool pdl = pdl_allowed(st, nullptr, 0, logprob, rows * 4);
+  const void* const out[4] = {logprob, entropy, top_ids, top_logprobs};
+  const size_t out_bytes[4] = {rows * 4, rows * 4, rows * top_k * 4, rows * top_k * 4};
+  const bool pdl = pdl_allowed_ranges(st, nullptr, nullptr, 0, out, out_bytes, 4);
   const cudaError_t e = launch_kernel_cluster(kernel, dim3(ctas, static_cast<unsigned>(rows)), dim3(THREADS), sizeof(LogprobShared), st, pdl, ctas, logits, targets, logprob,
                                               entropy, top_ids, top_logprobs, static_cast<uint32_t>(vocab), static_cast<int>(top_k), row_base);
   if (e != cudaSuccess) {

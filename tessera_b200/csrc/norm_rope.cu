@@ -239,8 +239,9 @@ struct Range {
   }
 };
 
-template <int OUT>
-int launch_norm_rope(NormRopeParams& p, uint64_t rows, bool vec, cudaStream_t st) {
+// out: everything the launch writes, which a projection behind it may read as its weights (an FP8 cache and its scales are gemm_fp8's)
+template <int OUT, int N>
+int launch_norm_rope(NormRopeParams& p, uint64_t rows, bool vec, const Range (&out)[N], cudaStream_t st) {
   constexpr bool kQuant = OUT == TSR_KV_INT8 || OUT == TSR_KV_INT4 || OUT == TSR_KV_FP8;
   // A warp a head while that does not fill the machine, then all of a row's query heads in one CTA: the row's angles are formed
   // once a CTA (512 rows, before the last step: 12.4 us, with a warp a head 14.5).
@@ -248,7 +249,10 @@ int launch_norm_rope(NormRopeParams& p, uint64_t rows, bool vec, cudaStream_t st
   p.heads_per_cta = (p.heads + parts - 1) / parts;
   const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(1 + parts));
   const size_t smem = kQuant ? static_cast<size_t>(p.kv_heads) * p.head_dim * 4 : 0;
-  const bool pdl = pdl_allowed(st, nullptr, 0, p.q_out, rows * p.heads * p.head_dim * 4);
+  const void* written[N];
+  size_t written_bytes[N];
+  for (int i = 0; i < N; ++i) written[i] = out[i].at, written_bytes[i] = out[i].bytes;
+  const bool pdl = pdl_allowed_ranges(st, nullptr, nullptr, 0, written, written_bytes, N);
   if (launch_kernel(vec ? qk_norm_rope_kernel<OUT, 4> : qk_norm_rope_kernel<OUT, 1>, grid, dim3(kNormThreads), smem, st, pdl, p) != cudaSuccess) {
     cudaGetLastError();
     return kDeviceError;
@@ -287,14 +291,14 @@ int qk_norm_rope(const float* q, const float* k, const float* q_w, const float* 
   // in place head by head, else apart: a head is read whole before it is written, another CTA's may not be there yet
   const uint64_t q_bytes = rows * heads * head_dim * 4, k_bytes = rows * kv_heads * head_dim * 4;
   const Range in[5] = {{q, q_bytes}, {k, k_bytes}, {q_w, head_dim * 4}, {k_w, head_dim * 4}, {pos, rows * 24}};
-  const Range qo{q_out, q_bytes}, ko{k_out, k_bytes};
+  const Range out[2] = {{q_out, q_bytes}, {k_out, k_bytes}}, &qo = out[0], &ko = out[1];
   if (qo.meets(ko)) return kInvalidArgument;
   for (const Range& r : in)
     if ((qo.meets(r) && !(r.at == q && q_out == q)) || (ko.meets(r) && !(r.at == k && k_out == k))) return kInvalidArgument;
   if (dry) return kOk;
   p.k_out = k_out;
   const bool vec = head_dim % 4 == 0 && rope_dim % 8 == 0 && wide(q) && wide(k) && wide(q_w) && wide(k_w) && wide(q_out) && wide(k_out);
-  return launch_norm_rope<kToFloat>(p, rows, vec, st);
+  return launch_norm_rope<kToFloat>(p, rows, vec, out, st);
 }
 
 int qk_norm_rope_append(int kv_format, const float* q, const float* k, const float* v, const float* q_w, const float* k_w, const uint64_t* pos,
@@ -325,7 +329,8 @@ int qk_norm_rope_append(int kv_format, const float* q, const float* k, const flo
   p.k_scale = quant ? k_scale + cache_row : nullptr, p.v_scale = quant ? v_scale + cache_row : nullptr;
   const uint64_t q_bytes = rows * heads * head_dim * 4, k_bytes = rows * cols * 4;
   const Range in[6] = {{q, q_bytes}, {k, k_bytes}, {v, k_bytes}, {q_w, head_dim * 4}, {k_w, head_dim * 4}, {pos, rows * 24}};
-  const Range out[5] = {{q_out, q_bytes}, {p.k_cache, rows * row_bytes}, {p.v_cache, rows * row_bytes}, {p.k_scale, rows * 4}, {p.v_scale, rows * 4}};
+  const uint64_t scale_bytes = quant ? rows * 4 : 0;
+  const Range out[5] = {{q_out, q_bytes}, {p.k_cache, rows * row_bytes}, {p.v_cache, rows * row_bytes}, {p.k_scale, scale_bytes}, {p.v_scale, scale_bytes}};
   for (int i = 0; i < 5; ++i) {
     for (const Range& r : in)
       if (out[i].meets(r) && !(i == 0 && r.at == q && q_out == q)) return kInvalidArgument;
@@ -336,11 +341,11 @@ int qk_norm_rope_append(int kv_format, const float* q, const float* k, const flo
                    (quant || (wide(p.k_cache) && wide(p.v_cache)));
   if (dry) return kOk;
   switch (kv_format) {
-    case TSR_KV_F32: return launch_norm_rope<TSR_KV_F32>(p, rows, vec, st);
-    case TSR_KV_F16: return launch_norm_rope<TSR_KV_F16>(p, rows, vec, st);
-    case TSR_KV_INT8: return launch_norm_rope<TSR_KV_INT8>(p, rows, vec, st);
-    case TSR_KV_INT4: return launch_norm_rope<TSR_KV_INT4>(p, rows, vec, st);
-    default: return launch_norm_rope<TSR_KV_FP8>(p, rows, vec, st);
+    case TSR_KV_F32: return launch_norm_rope<TSR_KV_F32>(p, rows, vec, out, st);
+    case TSR_KV_F16: return launch_norm_rope<TSR_KV_F16>(p, rows, vec, out, st);
+    case TSR_KV_INT8: return launch_norm_rope<TSR_KV_INT8>(p, rows, vec, out, st);
+    case TSR_KV_INT4: return launch_norm_rope<TSR_KV_INT4>(p, rows, vec, out, st);
+    default: return launch_norm_rope<TSR_KV_FP8>(p, rows, vec, out, st);
   }
 }
 
