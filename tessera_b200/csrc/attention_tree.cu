@@ -1005,8 +1005,8 @@ template <int D>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 attention_tree_merge_kernel(const float* __restrict__ pacc, const float* __restrict__ pmax, const float* __restrict__ psum,
                             float* __restrict__ out, int splits, int total) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   const int lane = threadIdx.x & 31;
   const size_t row = static_cast<size_t>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
   if (row >= static_cast<size_t>(total)) return;

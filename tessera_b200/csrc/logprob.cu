@@ -180,8 +180,8 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
     }
   };
   if (tid == 0) sh.count = 0;
-  pdl_trigger();
   pdl_wait();  // (this kernel's start overlaps the end of the one before it)
+  pdl_trigger();
   load(begin);
   float given = -INFINITY;  // the target's logit
   if (rank == 0 && tid == 0) {

@@ -121,9 +121,9 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_rope_kernel(const NormRo
     }
   };
   // (this kernel's start overlaps the end of the one before it, which may write anything that is read from here on)
-  pdl_trigger();
   const double freq = tid < pairs ? exp2(p.log2_theta * (-2.0 * tid / p.rope_dim)) : 0.0;
   pdl_wait();
+  pdl_trigger();
   load(h0 + warp);
   if (tid < pairs) {
     const unsigned long long at = p.pos[row * 3 + (tid < p.sec_t ? 0 : tid < p.sec_t + p.sec_h ? 1 : 2)];

@@ -61,3 +61,11 @@ def test_a_projection_over_rows_just_appended(which):
     want = t.passes(4, which, False, True)
     assert np.isfinite(want).all() and not np.array_equal(want[0], want[1])
     assert np.array_equal(t.passes(400, which, False, False), np.tile(want, (100, 1)))
+
+
+@pytest.mark.parametrize("which", [0, 1], ids=["keys", "values"])
+def test_a_projection_one_launch_after_the_append(which):
+    """The launch between them starts under the append, the projection under the launch between, but not under both."""
+    t = Append()
+    want = t.passes(4, which, False, True)
+    assert np.array_equal(t.passes(400, which, True, False), np.tile(want, (100, 1)))
