@@ -132,6 +132,7 @@ bool pdl_allowed_ranges(cudaStream_t stream, const void* const* reads, const siz
     if (slot->count < 0) ok = false;  // more outputs than the table holds: anything may have been written
   }
   if (slot == nullptr) {
+    if (nreads > 0) ok = false;  // a stream new to the table, or one that others have pushed out of it: what its last launch wrote is not known
     static int next = 0;
     slot = &table[next];
     next = (next + 1) % 16;
