@@ -322,7 +322,8 @@ int tsr_attention_combine(const float* pacc, const float* pmax, const float* psu
  * sees the past, its ancestors and itself, with window != 0 the last `window` of these.  A row with any other value, or
  * below one, is not used: it sees nothing, no row sees it, its result is 0 (trees smaller than m).  Query row i is row
  * row_base + i of q / out (out may be q); scale, head mapping, scales of the quantised formats and limits on head_dim and heads as
- * tsr_attention; m at most 256, else TSR_UNSUPPORTED_FEATURE.  out may not overlap anything but q in place. */
+ * tsr_attention; m at most 256, else TSR_UNSUPPORTED_FEATURE.  out may not overlap anything but q in place.  The keys are cut into
+ * chunks through a workspace of the stream; in a capture, where no call of the size came before on the stream, they are not. */
 int tsr_attention_tree(int kv_format, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                        const int32_t* parents, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
                        uint64_t head_dim, uint64_t row_base, uint64_t window, void* stream);
@@ -346,7 +347,8 @@ int tsr_qk_norm_rope_append(int kv_format, const float* q, const float* k, const
  * tsr_repeat_heads expands).  The state (heads x dk x dv) is read at s + sbase and written at s_out + sbase (which may be the same),
  * alpha and beta are read at abase + t * heads + h; no other overlap.  dk 64 or 128 and dv % 16 == 0, else
  * TSR_UNSUPPORTED_FEATURE.  Results agree with the row-by-row form to fp32 rounding; a value that is not finite spreads over its
- * head's rows from the 32 it lies in on. */
+ * head's rows from the 32 it lies in on.  Needs a workspace of the stream: TSR_UNSUPPORTED_FEATURE too in a capture, where no call
+ * of the size came before on the stream. */
 int tsr_delta_chunk_heads(const float* s, const float* k, const float* v, const float* q, float* o, const float* alpha,
                           const float* beta, float* s_out, uint64_t heads, uint64_t k_heads, uint64_t dk, uint64_t dv,
                           uint64_t rows, uint64_t sbase, uint64_t abase, void* stream);

@@ -1569,7 +1569,11 @@ int flush_pending(tsr_context* ctx) {
       // second appearance: capture the rewritten queue, keep it, replay it
       const uint64_t before = launch_counter().load();
       if (cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal) == cudaSuccess) {
-        const int rc = issue_queue(ctx, q);
+        int rc = kOk;
+        {
+          OwnCapture own;
+          rc = issue_queue(ctx, q);
+        }
         cudaGraph_t graph = nullptr;
         const cudaError_t ec = cudaStreamEndCapture(ctx->stream, &graph);
         cudaGraphExec_t exec = nullptr;

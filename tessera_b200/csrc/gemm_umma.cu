@@ -1008,50 +1008,9 @@ int ring_maps(int fmt, const void* w, uint64_t n, uint64_t k, RingMaps* out) {
   return kOk;
 }
 
-// Device scratch for the pre-converted activations, one buffer per (device, stream),
-// grown on demand and never freed before exit (a captured graph may hold the pointer).
-// Returns null when the stream is being captured and no large enough buffer exists yet:
-// the tiles then convert the activations themselves.  The memory comes from the
-// stream-ordered pool, so growing it never synchronises the device.
+// Scratch for the pre-converted activations.  Null (a capture before the first plain launch of the size): the tiles then
+// convert the activations themselves.
 unsigned char* activation_scratch(cudaStream_t st, size_t bytes) { return stream_scratch(st, bytes); }
-
-}  // namespace
-
-// `slot` separates users whose buffers are alive at the same time (0: the tile kernels'
-// operands and partial sums; 1: the fp32 copies around a bf16 projection; 2: attention's chunk partials; 3: the
-// binary16 tile's partial regions when it cuts k).
-unsigned char* stream_scratch(cudaStream_t st, size_t bytes, int slot) {
-  struct Entry {
-    int device;
-    int slot;
-    cudaStream_t stream;
-    unsigned char* ptr;
-    size_t bytes;
-  };
-  static std::mutex mutex;
-  static std::vector<Entry> table;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-  std::lock_guard<std::mutex> lock(mutex);
-  for (const Entry& e : table)
-    if (e.device == dev && e.slot == slot && e.stream == st && e.bytes >= bytes) return e.ptr;
-  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(st, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone) {
-    cudaGetLastError();
-    return nullptr;
-  }
-  size_t want = 4u << 20;
-  while (want < bytes) want <<= 1;
-  void* ptr = nullptr;
-  if (cudaMallocAsync(&ptr, want, st) != cudaSuccess) {
-    cudaGetLastError();
-    return nullptr;
-  }
-  table.push_back(Entry{dev, slot, st, static_cast<unsigned char*>(ptr), want});
-  return static_cast<unsigned char*>(ptr);
-}
-
-namespace {
 
 template <int FMT, bool RING>
 int launch_umma_impl(UmmaParams p, const RingMaps& maps, cudaStream_t st, bool allow_scratch) {

@@ -231,10 +231,19 @@ int umma_gemm(int fmt, const float* a, const void* w, const float* scale, float*
 int gemm_q4k_dispatch(const float* a, const void* w, float* c, uint64_t m, uint64_t n, uint64_t k,
                       uint64_t split, cudaStream_t st, bool allow_scratch);
 int umma_wait_timeouts(unsigned int* count);
-// Device scratch of a (device, stream) pair, grown on demand from the stream-ordered pool and
-// kept until exit (a captured graph may hold the pointer).  Null when the stream is being
-// captured and no large enough buffer exists yet.  Work on one stream uses it in stream order.
+// Device scratch of a (device, stream) pair (scratch.cu), grown on demand from the stream-ordered pool, so that growing it never
+// synchronises the device, and kept until exit.  Work on one stream uses it in stream order.  A captured launch gets a
+// buffer that its graph keeps, as graphs may be replayed on any stream; null where no plain launch of the size came before the
+// capture.  `slot` separates users whose buffers are alive at the same time: 0 the tile kernels' operands and partial sums, 1 the
+// fp32 copies around a bf16 projection, 2 attention's chunk partials, 3 the binary16 tile's partial regions when it cuts k, 4 the
+// delta rule's chunks, 5 the tree attention's chunk partials.
 unsigned char* stream_scratch(cudaStream_t st, size_t bytes, int slot = 0);
+// While one lives on a thread, the captures there are of a queue that is replayed on the stream it was captured on only: its
+// launches share the buffers of the stream's plain launches.
+struct OwnCapture {
+  OwnCapture();
+  ~OwnCapture();
+};
 // bf16 <-> fp32 copies on the stream (elementwise.cu); the fp32 -> bf16 direction rounds to nearest even
 int convert_bf16_to_f32(const void* src, float* dst, uint64_t n, cudaStream_t st);
 int convert_f32_to_bf16(const float* src, void* dst, uint64_t n, cudaStream_t st);
