@@ -729,13 +729,16 @@ template <int DK>
 int launch_delta_chunk(DeltaChunkParams p, cudaStream_t st) {
   using S = ChunkShape<DK>;
   using Z = ScanShape<DK>;
-  // long prompts in pieces of kMostChunks, which bound the workspace (48 heads over 16 key heads of 128: 147 MB)
-  const int rows = p.rows, most = min((rows + kChunk - 1) / kChunk, kMostChunks);
+  // Long prompts in pieces of kMostChunks, which bound the workspace.  It comes in three sizes, 4, 16 and 64 chunks, since a stream
+  // keeps the smaller ones when it grows (48 heads over 16 key heads of 128: 9, 37 and 149 MB).
+  const int rows = p.rows;
+  int most = 4;
+  while (most < kMostChunks && most * kChunk < rows) most *= 4;
   const size_t key_bytes = static_cast<size_t>(p.k_heads) * most * 2 * S::kKeyBytes;
   const size_t mat_bytes = static_cast<size_t>(p.heads) * most * Z::kOutBytes;
   const size_t factor_bytes = static_cast<size_t>(p.heads) * most * sizeof(Factors);
   const size_t u_bytes = static_cast<size_t>(p.heads) * most * kChunk * p.dv * 4;
-  unsigned char* scratch = stream_scratch(st, key_bytes + mat_bytes + u_bytes + factor_bytes, 4);
+  unsigned char* scratch = stream_scratch(st, key_bytes + mat_bytes + u_bytes + factor_bytes, kScratchDelta);
   if (scratch == nullptr) return kUnsupportedFeature;  // a capture before the first plain launch of this size
   p.keys = scratch, p.mats = scratch + key_bytes;
   p.u = reinterpret_cast<float4*>(scratch + key_bytes + mat_bytes);

@@ -237,6 +237,7 @@ int umma_wait_timeouts(unsigned int* count);
 // capture.  `slot` separates users whose buffers are alive at the same time: 0 the tile kernels' operands and partial sums, 1 the
 // fp32 copies around a bf16 projection, 2 attention's chunk partials, 3 the binary16 tile's partial regions when it cuts k, 4 the
 // delta rule's chunks, 5 the tree attention's chunk partials.
+constexpr int kScratchDelta = 4;
 unsigned char* stream_scratch(cudaStream_t st, size_t bytes, int slot = 0);
 // While one lives on a thread, the captures there are of a queue that is replayed on the stream it was captured on only: its
 // launches share the buffers of the stream's plain launches.

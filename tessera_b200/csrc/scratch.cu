@@ -10,6 +10,9 @@
 namespace tsr {
 namespace {
 
+constexpr size_t kStep = 2u << 20;
+size_t in_steps(size_t bytes) { return (bytes + kStep - 1) / kStep * kStep; }
+
 struct Buffer {
   int device, slot;
   cudaStream_t stream;
@@ -54,8 +57,7 @@ unsigned char* capture_scratch(int dev, cudaStream_t st, size_t bytes, int slot)
     cudaGetLastError();
     return nullptr;
   }
-  constexpr size_t kStep = 2u << 20;
-  const size_t want = (bytes + kStep - 1) / kStep * kStep;
+  const size_t want = in_steps(bytes);
   Buffer b{dev, slot, st, id, nullptr, want};
   GraphBuffers& all = graph_buffers();
   {
@@ -132,7 +134,9 @@ unsigned char* stream_scratch(cudaStream_t st, size_t bytes, int slot) try {
     if (plain != nullptr && (!capturing || own_capture)) return plain;
     if (capturing && plain == nullptr) return nullptr;
     if (!capturing) {
-      size_t want = 4u << 20;
+      // twice as large every time, so that what a stream outgrew is no more than what it uses (the delta rule's come in few
+      // sizes already)
+      size_t want = slot == kScratchDelta ? in_steps(bytes) : 4u << 20;
       while (want < bytes) want <<= 1;
       void* ptr = nullptr;
       if (cudaMallocAsync(&ptr, want, st) != cudaSuccess) {

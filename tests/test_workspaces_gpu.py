@@ -120,3 +120,19 @@ def test_buffers_of_dropped_graphs_serve_later_ones():
         torch.cuda.synchronize()
         free.append(torch.cuda.mem_get_info()[0])
     assert free[5] - free[-1] < 8 << 20  # (a buffer is 8 MB and more)
+
+
+def test_prompts_that_grow():
+    """What a stream keeps after prompts of one to 64 chunks of rows: not much more than the largest needs."""
+    heads, k_heads, d, rows = 48, 16, 128, 64 * 32
+    new = lambda *shape: torch.full(shape, 0.01, device="cuda")
+    s, k, v, gates, o = new(heads, d, d), new(rows, k_heads, d), new(rows, heads, d), new(rows, heads), new(rows, heads, d)
+    stream, lib = torch.cuda.Stream(), capi.load_library()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for n in range(20, rows + 1, 60):
+        assert lib.tsr_delta_chunk_heads(s.data_ptr(), k.data_ptr(), v.data_ptr(), k.data_ptr(), o.data_ptr(), gates.data_ptr(), gates.data_ptr(),
+                                         s.data_ptr(), heads, k_heads, d, d, n, 0, 0, stream.cuda_stream) == 0
+    torch.cuda.synchronize()
+    chunk = k_heads * 2 * 32 * 4 * d + heads * (32 * 4 * d + 32 * 4 * 32 + 32 * d * 4 + 1024)  # keys and queries; W, P, u, factors
+    assert free - torch.cuda.mem_get_info()[0] < 64 * chunk * 1.75
