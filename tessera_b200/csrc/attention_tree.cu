@@ -145,6 +145,9 @@ constexpr int kScaleBufs = 4;
 constexpr int kNoExponent = -1000;
 constexpr int kUnused = 0x7FFFFFFF;
 constexpr int kWideScales = 16;  // exponents apart
+// Of the values' scales where weights are formed: a weight is at most 2^(14 - e), and 32 of them a thread have a finite sum (a tile of zero
+// values alone, as of a cache that has just been cleared, would give 2^124 each).
+constexpr int kLowestExponent = -107;
 
 struct TcParams {
   TreeParams t;
@@ -530,7 +533,8 @@ struct TcLoader {
       const int e = mine == 0 ? 0 : max(-110, min(114, static_cast<int>(mine >> 23) - 127 - 13));
       const float up = power_of_two(-e);
       if (mine != 0) high = max(high, e), low = min(low, e);
-      if (lane < 8) sh.scale[t % kScaleBufs][values ? 1 : 0][group * 8 + key] = power_of_two(e);
+      // (0 for a row of zeros: its weight, which is relative to the other rows' scales, may be large)
+      if (lane < 8) sh.scale[t % kScaleBufs][values ? 1 : 0][group * 8 + key] = mine == 0 ? 0.0f : power_of_two(e);
 #pragma unroll 4
       for (int it = 0; it < D / 32; ++it) {
         const int c = it * 4 + (lane >> 3);
@@ -797,7 +801,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tree_tc_kernel(const 
           most = fmaxf(most, sh.weighed[half ^ 1][row]);
           e = static_cast<int>(fminf(fmaxf(ceilf(most), -110.0f), 110.0f));
         }
-        e = max(-110, min(110, e));
+        e = max(kLowestExponent, min(110, e));
       }
       const float shift = now == kNoKey ? 0.0f : static_cast<float>(14 - e) - now;
       uint32_t hi[16], lo[16];
