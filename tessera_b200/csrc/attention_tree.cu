@@ -145,9 +145,9 @@ constexpr int kScaleBufs = 4;
 constexpr int kNoExponent = -1000;
 constexpr int kUnused = 0x7FFFFFFF;
 constexpr int kWideScales = 16;  // exponents apart
-// Of the values' scales where weights are formed: a weight is at most 2^(14 - e), and 32 of them a thread have a finite sum (a tile of zero
+// Of the values' scales where weights are formed: a weight is at most 2^(14 - e), and a thread's 32 have a finite sum (a tile of zero
 // values alone, as of a cache that has just been cleared, would give 2^124 each).
-constexpr int kLowestExponent = -107;
+constexpr int kLowestExponent = -108;
 
 struct TcParams {
   TreeParams t;
@@ -530,11 +530,11 @@ struct TcLoader {
       const int j = min(c0 + t * kTcKeys + group * 8 + key, c1 - 1);
       const bool zero = j >= p.t.n && unseen(j);
       if (zero) mine = 0;
-      const int e = mine == 0 ? 0 : max(-110, min(114, static_cast<int>(mine >> 23) - 127 - 13));
+      // (a row of zeros has the smallest scale: its weight, which is relative to the other rows' scales, may be large)
+      const int e = mine == 0 ? -126 : max(-110, min(114, static_cast<int>(mine >> 23) - 127 - 13));
       const float up = power_of_two(-e);
       if (mine != 0) high = max(high, e), low = min(low, e);
-      // (0 for a row of zeros: its weight, which is relative to the other rows' scales, may be large)
-      if (lane < 8) sh.scale[t % kScaleBufs][values ? 1 : 0][group * 8 + key] = mine == 0 ? 0.0f : power_of_two(e);
+      if (lane < 8) sh.scale[t % kScaleBufs][values ? 1 : 0][group * 8 + key] = power_of_two(e);
 #pragma unroll 4
       for (int it = 0; it < D / 32; ++it) {
         const int c = it * 4 + (lane >> 3);

@@ -75,3 +75,48 @@ def test_tiles_of_zero_values_among_others(kind):
     y = Timed(t)
     y.call()
     assert near_rows(y.out.cpu().numpy(), t.want())
+
+
+@pytest.mark.parametrize("kind,exponent", [("f32", 80), ("f32", 92), ("q8", 92), ("q4", 92), ("fp8", 92)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_large_keys_and_small_queries(kind, exponent, sign):
+    """Products of query and key are ordinary numbers, key by key in 32 bits as well; here all scores of a row are of one sign."""
+    t = Tree(kind, 5, 300, 12, 2, 128, seed=4)
+    t.q = np.abs(t.q).clip(0.3, 3.0)
+    lift = np.float32(2.0 ** exponent)
+    if t.ks is None:
+        t.k = np.abs(t.k) * sign
+        t.k[::3] *= lift
+        t.k[1::3] *= lift * 2
+        t.k[2::3] *= lift / 2
+    else:
+        codes = t.k.view(np.int8)
+        if kind == "q8":
+            t.k = (np.abs(codes.astype(np.int16)).clip(0, 127) * sign).astype(np.int8).view(np.uint8)
+        elif kind == "q4":
+            nibble = 3 if sign > 0 else 13
+            t.k = np.where(np.arange(t.k.size).reshape(t.k.shape) % 5 < 3, nibble, nibble << 4).astype(np.uint8)
+        else:
+            t.k = (t.k & 0x7F) | (0x80 if sign < 0 else 0)
+            t.k = t.k.astype(np.uint8)
+        t.ks = (t.ks * lift).astype(np.float32)
+    t.q = (t.q / lift / 16).astype(np.float32)
+    assert np.all(np.abs(t.q) > 2.0 ** -126)
+    y = Timed(t)
+    y.call()
+    # scores of either size: a weight's error is that of a score of up to 16, 16 2^-24 sqrt(128) / 8 and less
+    assert near_rows(y.out.cpu().numpy(), t.want(), 4e-5)
+
+
+@pytest.mark.parametrize("kind", ["f32", "q8", "q4", "fp8"])
+@pytest.mark.parametrize("exponent", [100, 112, -100, -110])
+def test_values_at_the_ends_of_their_range(kind, exponent):
+    t = Tree(kind, 9, 200, 12, 2, 128, seed=6)
+    lift = np.float32(2.0 ** exponent)
+    if t.vs is None:
+        t.v *= lift
+    else:
+        t.vs *= lift
+    y = Timed(t)
+    y.call()
+    assert near_rows(y.out.cpu().numpy(), t.want())
