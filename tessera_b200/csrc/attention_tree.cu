@@ -1142,6 +1142,8 @@ int attention_tree(int kv_format, const float* q, const void* k, const void* v, 
       head_dim == 0 || heads % kv_heads != 0 || row_base > 0x7FFFFFFFull || window > 0x7FFFFFFFull || kv_format < TSR_KV_F32 || kv_format > TSR_KV_FP8)
     return kInvalidArgument;
   if (kv_format >= TSR_KV_INT8 && (!k_scale || !v_scale)) return kInvalidArgument;
+  const uintptr_t item = kv_format == TSR_KV_F32 ? 4 : kv_format == TSR_KV_F16 ? 2 : 1;  // what the cache is read by at least
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % item != 0) return kInvalidArgument;
   if (m > kTreeRows || (head_dim != 128 && head_dim != 256) || heads / kv_heads > kAttnMaxGroup) return kUnsupportedFeature;
   const size_t skip = row_base * heads * head_dim;
   {  // a row's result is written while other rows are read; over its own queries it may go

@@ -69,3 +69,14 @@ def test_logprob_refusals(lib, mem):
     for bad in (dict(x=None), dict(targets=None), dict(lp=None), dict(ent=None), dict(ids=None), dict(tops=None), dict(rows=0), dict(vocab=0), dict(k=33),
                 dict(vocab=HUGE), dict(rows=HUGE)):
         assert call(**bad) == BAD, bad
+
+
+def test_tree_over_a_cache_off_its_elements_boundary(lib, mem):
+    """A binary16 or fp32 cache has to lie on its elements' boundary (bytes may lie anywhere)."""
+    p = mem[0]
+
+    def call(fmt, k, v):
+        return lib.tsr_attention_tree(fmt, p[0], k, v, p[3], p[4], p[5], p[6], 4, 16, 4, 2, 128, 0, 0, None)
+
+    for fmt, off in ((0, 1), (0, 2), (1, 1)):
+        assert call(fmt, p[1] + off, p[2]) == BAD and call(fmt, p[1], p[2] + off) == BAD
