@@ -293,8 +293,8 @@ int qk_norm_rope(const float* q, const float* k, const float* q_w, const float* 
   const Range in[5] = {{q, q_bytes}, {k, k_bytes}, {q_w, head_dim * 4}, {k_w, head_dim * 4}, {pos, rows * 24}};
   const Range out[2] = {{q_out, q_bytes}, {k_out, k_bytes}}, &qo = out[0], &ko = out[1];
   if (qo.meets(ko)) return kInvalidArgument;
-  for (const Range& r : in)
-    if ((qo.meets(r) && !(r.at == q && q_out == q)) || (ko.meets(r) && !(r.at == k && k_out == k))) return kInvalidArgument;
+  for (int i = 0; i < 5; ++i)  // (by its place: keys or weights may lie where the queries do)
+    if ((qo.meets(in[i]) && !(i == 0 && q_out == q)) || (ko.meets(in[i]) && !(i == 1 && k_out == k))) return kInvalidArgument;
   if (dry) return kOk;
   p.k_out = k_out;
   const bool vec = head_dim % 4 == 0 && rope_dim % 8 == 0 && wide(q) && wide(k) && wide(q_w) && wide(k_w) && wide(q_out) && wide(k_out);
@@ -332,8 +332,8 @@ int qk_norm_rope_append(int kv_format, const float* q, const float* k, const flo
   const uint64_t scale_bytes = quant ? rows * 4 : 0;
   const Range out[5] = {{q_out, q_bytes}, {p.k_cache, rows * row_bytes}, {p.v_cache, rows * row_bytes}, {p.k_scale, scale_bytes}, {p.v_scale, scale_bytes}};
   for (int i = 0; i < 5; ++i) {
-    for (const Range& r : in)
-      if (out[i].meets(r) && !(i == 0 && r.at == q && q_out == q)) return kInvalidArgument;
+    for (int j = 0; j < 6; ++j)
+      if (out[i].meets(in[j]) && !(i == 0 && j == 0 && q_out == q)) return kInvalidArgument;
     for (int j = 0; j < i; ++j)
       if (out[i].meets(out[j])) return kInvalidArgument;
   }

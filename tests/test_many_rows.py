@@ -80,3 +80,19 @@ def test_tree_over_a_cache_off_its_elements_boundary(lib, mem):
 
     for fmt, off in ((0, 1), (0, 2), (1, 1)):
         assert call(fmt, p[1] + off, p[2]) == BAD and call(fmt, p[1], p[2] + off) == BAD
+
+
+def test_queries_that_are_the_keys(lib, mem):
+    """In place over queries that the keys (or the weights) are read from as well: another CTA may read them after they are written."""
+    p = mem[0]
+
+    def call(q=p[0], k=p[1], qw=p[2], kw=p[3], qo=p[5], ko=p[6]):
+        return lib.tsr_qk_norm_rope(q, k, qw, kw, p[4], qo, ko, 2, 1, 1, 64, 32, 1e6, 6, 5, 5, 1e-6, None)
+
+    def append(q=p[0], k=p[1], v=p[7], qw=p[2], qo=p[5]):
+        return lib.tsr_qk_norm_rope_append(0, q, k, v, qw, p[3], p[4], qo, p[8], p[9], None, None, 2, 0, 1, 1, 64, 32, 1e6, 6, 5, 5, 1e-6, None)
+
+    for bad in (dict(k=p[0], qo=p[0]), dict(k=p[0], ko=p[0]), dict(qw=p[0], qo=p[0]), dict(kw=p[1], ko=p[1]), dict(qw=p[1], ko=p[1])):
+        assert call(**bad) == BAD, bad
+    for bad in (dict(k=p[0], qo=p[0]), dict(v=p[0], qo=p[0]), dict(qw=p[0], qo=p[0])):
+        assert append(**bad) == BAD, bad
