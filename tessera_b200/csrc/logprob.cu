@@ -419,13 +419,13 @@ int logprob_rows(const float* logits, const uint32_t* targets, float* logprob, f
           out[4] = {{logprob, rows * 4}, {entropy, rows * 4}, {top_ids, rows * top_k * 4}, {top_logprobs, rows * top_k * 4}};
   auto meet = [](const auto& a, const auto& b) {
     const auto *x = static_cast<const unsigned char*>(a.at), *y = static_cast<const unsigned char*>(b.at);
-    return x < y + b.bytes && y < x + a.bytes;
+    return a.bytes != 0 && x < y + b.bytes && y < x + a.bytes;
   };
   for (int i = 0; i < 4; ++i) {  // a row's results are written while others are read
     for (const auto& r : in)
       if (meet(out[i], r)) return kInvalidArgument;
     for (int j = 0; j < i; ++j)
-      if (meet(out[i], out[j])) return kInvalidArgument;
+      if (out[j].bytes != 0 && meet(out[i], out[j])) return kInvalidArgument;
   }
   if (dry) return kOk;
   // CTAs of a row: while the machine has room for them (two a SM; clusters of sixteen, of which a GPC holds few, one a SM) and each

@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 from tessera_b200 import capi
 
@@ -96,3 +97,12 @@ def test_queries_that_are_the_keys(lib, mem):
         assert call(**bad) == BAD, bad
     for bad in (dict(k=p[0], qo=p[0]), dict(v=p[0], qo=p[0]), dict(qw=p[0], qo=p[0])):
         assert append(**bad) == BAD, bad
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the call would run")
+def test_logprob_without_a_top_list_overlaps_nothing_there(lib, mem):
+    """With no top list its places are not written, whatever they are."""
+    p = mem[0]
+    call = lambda k, at: lib.tsr_logprob_rows(p[0], p[1], p[2], p[3], at, at, 2, 10, k, 0, None)
+    assert call(2, p[0] + 16) == BAD
+    assert call(0, p[0] + 16) not in (BAD, NOT_SERVED)  # (accepted: what fails without a GPU is the launch)
