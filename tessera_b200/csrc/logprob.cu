@@ -26,16 +26,14 @@
 
 #include "codec.cuh"
 #include "launch.h"
+#include "logprob_plan.h"
 #include "tessera_b200.h"
 
 namespace tsr {
 namespace {
 
-constexpr int kLpMost = 512;    // threads of a CTA at most
-constexpr int kLpPer = 12;      // logits of a thread at a time
 constexpr int kLpList = 1024;   // entries of the list
 constexpr int kLpTop = 32;      // top_k at most, as top_k_rows
-constexpr int kLpCluster = 16;  // CTAs of a row at most
 constexpr int kLpCut = 96;      // entries from which the list is cut back before the next tile
 static_assert(kLpCluster * kLpTop <= kLpMost && kLpCut > kLpTop, "a thread an entry where the CTAs meet");
 
@@ -375,24 +373,40 @@ logprob_rows_kernel(const float* __restrict__ logits, const uint32_t* __restrict
   }
 }
 
+// How many clusters of `ctas` CTAs (a power of two) the device runs at a time.
 template <int VEC, int THREADS>
-int launch_logprob(unsigned ctas, uint64_t rows, const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids,
+int logprob_resident(unsigned ctas) {
+  static std::atomic<int> known[64][5];  // the number plus one; 0: not asked
+  int dev = 0, log = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  while ((1u << log) < ctas) ++log;
+  if (const int v = known[dev][log].load(std::memory_order_relaxed)) return v - 1;
+  const auto kernel = logprob_rows_kernel<VEC, THREADS>;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = ctas;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = sizeof(LogprobShared);
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  int clusters = 0;
+  if ((ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
+    cudaGetLastError();
+    clusters = 0;
+  }
+  known[dev][log].store(clusters + 1, std::memory_order_relaxed);
+  return clusters;
+}
+
+template <int VEC, int THREADS>
+int launch_logprob(uint64_t rows, const float* logits, const uint32_t* targets, float* logprob, float* entropy, uint32_t* top_ids,
                    float* top_logprobs, uint64_t vocab, uint64_t top_k, uint64_t row_base, cudaStream_t st) {
   const auto kernel = logprob_rows_kernel<VEC, THREADS>;
-  if (ctas > 8) {  // clusters beyond the portable size
-    static std::atomic<unsigned long long> allowed{0};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return kDeviceError;
-    const unsigned long long bit = 1ull << (dev & 63);
-    if ((allowed.load() & bit) == 0) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-        cudaGetLastError();
-        ctas = 8;
-      } else {
-        allowed.fetch_or(bit);
-      }
-    }
-  }
+  const unsigned ctas = logprob_ctas(rows, vocab, logprob_resident<VEC, THREADS>);
   const void* const out[4] = {logprob, entropy, top_ids, top_logprobs};
   const size_t out_bytes[4] = {rows * 4, rows * 4, rows * top_k * 4, rows * top_k * 4};
   const bool pdl = pdl_allowed_ranges(st, nullptr, nullptr, 0, out, out_bytes, 4);
@@ -428,13 +442,9 @@ int logprob_rows(const float* logits, const uint32_t* targets, float* logprob, f
       if (out[j].bytes != 0 && meet(out[i], out[j])) return kInvalidArgument;
   }
   if (dry) return kOk;
-  // CTAs of a row: while the machine has room for them (two a SM; clusters of sixteen, of which a GPC holds few, one a SM) and each
-  // has a quarter of a tile.
-  unsigned ctas = 1;
-  while (ctas < kLpCluster && rows * (ctas * 2) <= (ctas < 8 ? 296 : 148) && vocab / (ctas * 2) >= kLpMost * kLpPer / 4) ctas *= 2;
   const bool wide = vocab % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15u) == 0;
-  return wide ? launch_logprob<4, kLpMost>(ctas, rows, logits, targets, logprob, entropy, top_ids, top_logprobs, vocab, top_k, row_base, st)
-              : launch_logprob<1, kLpMost>(ctas, rows, logits, targets, logprob, entropy, top_ids, top_logprobs, vocab, top_k, row_base, st);
+  return wide ? launch_logprob<4, kLpMost>(rows, logits, targets, logprob, entropy, top_ids, top_logprobs, vocab, top_k, row_base, st)
+              : launch_logprob<1, kLpMost>(rows, logits, targets, logprob, entropy, top_ids, top_logprobs, vocab, top_k, row_base, st);
 }
 
 }  // namespace tsr
