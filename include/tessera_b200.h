@@ -322,8 +322,11 @@ int tsr_attention_combine(const float* pacc, const float* pmax, const float* psu
  * sees the past, its ancestors and itself, with window != 0 the last `window` of these.  A row with any other value, or
  * below one, is not used: it sees nothing, no row sees it, its result is 0 (trees smaller than m).  Query row i is row
  * row_base + i of q / out (out may be q); scale, head mapping, scales of the quantised formats and limits on head_dim and heads as
- * tsr_attention; m at most 256, else TSR_UNSUPPORTED_FEATURE.  out may not overlap anything but q in place.  The keys are cut into
- * chunks through a workspace of the stream; in a capture, where no call of the size came before on the stream, they are not. */
+ * tsr_attention; m at most 256, else TSR_UNSUPPORTED_FEATURE.  fp32 and fp16 caches lie on their elements' boundary.  Where q, k, v
+ * and out do not all lie on 16 bytes a kernel key by key serves the call (3 to 14 times as long for few rows or keys, more
+ * for long ones).  out may not overlap anything but q in place.  The keys are cut into
+ * chunks through a workspace of the stream; in a capture, where no call of the size came before on the stream, they are not
+ * (64 rows behind 32768 FP8 keys: 1525 us instead of 151). */
 int tsr_attention_tree(int kv_format, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                        const int32_t* parents, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
                        uint64_t head_dim, uint64_t row_base, uint64_t window, void* stream);
@@ -346,13 +349,15 @@ int tsr_qk_norm_rope_append(int kv_format, const float* q, const float* k, const
  * and chains of drafted tokens.  Queries and keys are rows x k_heads x dk: value head h reads key head h % k_heads (what
  * tsr_repeat_heads expands).  The state (heads x dk x dv) is read at s + sbase and written at s_out + sbase (which may be the same),
  * alpha and beta are read at abase + t * heads + h; no other overlap.  dk 64 or 128 and dv % 16 == 0, else
- * TSR_UNSUPPORTED_FEATURE.  Results agree with the row-by-row form to fp32 rounding; a value that is not finite spreads over its
- * head's rows from the 32 it lies in on.  Needs a workspace of the stream: TSR_UNSUPPORTED_FEATURE too in a capture, where no call
+ * TSR_UNSUPPORTED_FEATURE.  Only the last row's state is left: a host that may take back some of the rows, as after a chain that
+ * is accepted in part, needs tsr_delta_step_heads with sstride != 0 or runs the accepted rows again from s.  Results agree with the
+ * row-by-row form to a few 2^-23 of the largest values of the 32 rows a row lies among (also where a decay of 0 parts them); a value that
+ * is not finite spreads over its head's rows from the 32 it lies in on.  Needs a workspace of the stream: TSR_UNSUPPORTED_FEATURE too in a capture, where no call
  * of the size came before on the stream. */
 int tsr_delta_chunk_heads(const float* s, const float* k, const float* v, const float* q, float* o, const float* alpha,
                           const float* beta, float* s_out, uint64_t heads, uint64_t k_heads, uint64_t dk, uint64_t dv,
                           uint64_t rows, uint64_t sbase, uint64_t abase, void* stream);
-/* logprob_rows (this library's own): of rows x vocab logits (output row r: input row row_base + r) the log probability of
+/* logprob_rows (this library's own): of rows (at most 65535) x vocab logits (output row r: input row row_base + r) the log probability of
  * targets[r] (-inf for an id >= vocab), the entropy (nats) and the top_k (0..32; 0: top_ids and top_logprobs may be null) largest
  * logits' indices and log probabilities, descending, equal logits lowest index first.  A logit of -inf is a token that cannot
  * come; a row of nothing else gives -inf and entropy 0; a row with NaN or +inf gives NaN.  Places beyond the vocabulary: id 0, -inf. */

@@ -134,10 +134,12 @@ __global__ void __launch_bounds__(kTreeWarps * 32) attention_tree_rows_kernel(co
 // Measured, 24 heads over 4 of 256 unless said: FP8, 16 rows behind 512 18.1 us; fp16, 61 rows behind 4000, 16 heads over 2 of 128
 // 25 us; fp32, 8 rows behind 4096 36 us; FP8, 64 rows behind 32768 151 us (the MMAs' operations alone 31 us).
 // A kernel key by key (as attention_tree_rows_kernel) took 61, 391, 981 and 10389 us.  What bounds: one tile costs 12 us
-// (tensor memory, paths, two terms of the queries, the first scores) and the second launch, which joins the chunks, 3 to 4; a
-// long row of tiles the issue of its MMAs, 48 a tile of about 70 clocks whatever their width (tensor pipe 42 % busy); the fp32 cache
-// its loaders, which scale and split every row (9 us a tile; 12 with stores of a row at a time, 16 of them to the same banks).  Tiles of 64 keys, since two tiles' weights lie over their scores and columns
-// of tensor memory are short.  Bytes by bulk copies of a key each 295 us for the long case, by tiled copies 152.
+// (tensor memory, paths, two terms of the queries, the first scores) and the second launch, which joins the chunks, 3 to 4.  In a
+// long row of tiles one takes 5900 clocks, of which the issuing thread spends 3300 on its 48 MMAs (2900 by their rates: 55 clocks
+// with 64 columns, 70 with 128) and waits 730 for a half of the outputs to be read, both halves having one accumulator, and 1250
+// for keys, weights, values and the last outputs (tensor pipe 42 % busy).  The fp32 cache: its loaders, which scale and split
+// every row (9 us a tile; 12 with stores of a row at a time, 16 of them to the same banks).  Tiles of 64 keys, since two tiles'
+// weights lie over their scores and columns of tensor memory are short.  Bytes by bulk copies of a key each 295 us for the long case, by tiled copies 152.
 constexpr int kSoftThreads = 256, kLoadThreads = 96, kTcThreads = kSoftThreads + kLoadThreads + 32;
 constexpr int kTcRows = 128, kTcKeys = 64;
 constexpr uint32_t kColQ = 0, kColS = 256, kColO = 384;  // of tensor memory; tile t's scores and weights: kColS + 64 (t % 2)

@@ -19,7 +19,7 @@
 // Bound: the chain of the chunks.  48 heads over 16 key heads of 128 x 128, 33 rows: 16 us; 512 rows: 63 us, of which 22 the first kernel (44 % of
 // its issue slots, a chain of short phases) and 48 the scan, 2.9 us a chunk; 32 heads, 2048 rows: 179 us, 61 and 128, 2.0 us a chunk
 // (tensor pipe 30 % busy, a third of the issue slots: what a warp waits for is its own last instruction).  Row by row the same
-// takes 155 us for 512 rows.  Steps: one warp for 16 whole columns, outputs by the same warp 78 and 261; outputs by warps of
+// takes 155 us for 512 rows; 33 rows 25 us with the two repeat_heads that it needs, one row 11 us against 13 here, two rows 14.  Steps: one warp for 16 whole columns, outputs by the same warp 78 and 261; outputs by warps of
 // their own, copies of 16 bytes by all threads 75 and 270 (the copies' issue held up everybody); T folded into W, half of dk a
 // warp 82 and 260; bulk copies by one thread 75 and 235; u as a bulk copy too, operands of the MMAs a step ahead 68 and 186.
 #include <cuda_fp16.h>
@@ -367,7 +367,9 @@ __global__ void __launch_bounds__(kPrepThreads, PER_SM) delta_chunk_prepare_kern
           for (int c = 0; c < 2; ++c) two_terms(x[step][r][2 * c] * up[r], x[step][r][2 * c + 1] * up[r], ah[step][2 * c + r], al[step][2 * c + r]);
     };
     for (int w = 0; w < heads; ++w) {
-      if (warp < 4) {  // W: 16 rows by half of the elements a warp
+      // W: 16 rows by half of the elements a warp.  Large and small products share an accumulator: there are two steps of them, and
+      // accumulators of their own left the results' errors as they were (2.3e-7, 2.9e-7) and spilled (512 rows: 64.8 us against 63.1).
+      if (warp < 4) {
         const int half = warp & 1, m = warp >> 1;
         constexpr int kTiles = DK / 16;
         uint32_t ah[2][4], al[2][4];

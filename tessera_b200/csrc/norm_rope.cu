@@ -12,8 +12,8 @@
 // maximum over all kv heads), the other CTAs the query heads.
 //
 // Bound: for few rows the launch and one head's chain (16 rows of 24 + 4 heads of 256, FP8 cache: 5.7 us in the kernel, 6.4 us a
-// call), for many the issue slots (512 rows, fp16 cache: 8.8 us, of which 1.5 under the launch before; half of them taken; the
-// bytes alone 4.8 us).  There four elements
+// call), for many the barrier behind the angles, which one warp of a CTA forms in double precision while the others wait (512
+// rows, fp16 cache: 8.8 us, of which 1.5 under the launch before; half of the issue slots taken; the bytes alone 4.8 us).  There four elements
 // at a time in the rotation, a head's norm ahead of the barrier that the angles need and the next head's elements under way
 // brought 12.3 to 10.3 us; registers cut for more CTAs an SM cost (48: 12.4, 40: 14.5 us, spilled), and so did a table of
 // frequencies from the host (1.2 us a call).
