@@ -16,6 +16,7 @@
 
 #include "context.h"
 #include "launch.h"
+#include "launch_record.h"
 #include "tessera_b200.h"
 
 namespace {
@@ -101,55 +102,23 @@ unsigned char* tsr_context::window(int* index) {
 
 namespace tsr {
 
-// Output ranges written by the last launch of this library, per stream.
 bool pdl_allowed_ranges(cudaStream_t stream, const void* const* reads, const size_t* read_bytes, int nreads,
                         const void* const* writes, const size_t* write_bytes, int nwrites) {
   static const bool enabled = [] {
     const char* v = std::getenv("TSR_PDL");
     return v == nullptr || std::atoi(v) != 0;
   }();
-  constexpr int kRanges = 12;
-  struct Last {
-    cudaStream_t stream;
-    bool used;
-    int count;
-    const unsigned char* ptr[kRanges];
-    size_t bytes[kRanges];
-  };
   static std::mutex mutex;
-  static Last table[16] = {};
+  static LaunchRecord record;
+  int device = 0;
+  cudaGetDevice(&device);
   std::lock_guard<std::mutex> lock(mutex);
-  Last* slot = nullptr;
-  for (Last& l : table)
-    if (l.used && l.stream == stream) slot = &l;
-  bool ok = enabled;
-  if (slot != nullptr) {
-    for (int i = 0; i < nreads; ++i) {
-      const auto* r = static_cast<const unsigned char*>(reads[i]);
-      for (int j = 0; j < slot->count; ++j)
-        if (r < slot->ptr[j] + slot->bytes[j] && slot->ptr[j] < r + read_bytes[i]) ok = false;  // previous output is our weight
-    }
-    if (slot->count < 0) ok = false;  // more outputs than the table holds: anything may have been written
-  }
-  if (slot == nullptr) {
-    if (nreads > 0) ok = false;  // a stream new to the table, or one that others have pushed out of it: what its last launch wrote is not known
-    static int next = 0;
-    slot = &table[next];
-    next = (next + 1) % 16;
-  }
-  slot->stream = stream;
-  slot->used = true;
-  slot->count = nwrites <= kRanges ? nwrites : -1;
-  for (int j = 0; j < slot->count; ++j) {
-    slot->ptr[j] = static_cast<const unsigned char*>(writes[j]);
-    slot->bytes[j] = write_bytes[j];
-  }
-  return ok;
+  return record.next(device, stream, reads, read_bytes, nreads, writes, write_bytes, nwrites) && enabled;
 }
 
 bool pdl_allowed(cudaStream_t stream, const void* read_ptr, size_t read_bytes, const void* out_ptr,
                  size_t out_bytes) {
-  return pdl_allowed_ranges(stream, &read_ptr, &read_bytes, 1, &out_ptr, &out_bytes, 1);
+  return pdl_allowed_ranges(stream, &read_ptr, &read_bytes, read_bytes != 0 ? 1 : 0, &out_ptr, &out_bytes, 1);
 }
 
 int allow_dynamic_smem(const void* kernel, int bytes) {

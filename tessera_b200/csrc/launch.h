@@ -122,7 +122,8 @@ inline cudaError_t launch_kernel_cluster(void (*kernel)(KArgs...), dim3 grid, di
 int allow_dynamic_smem(const void* kernel, int bytes);
 
 // Multi-range form of pdl_allowed (a launch over several weight tensors): true when none of the
-// `reads` ranges overlaps a range the previous launch of this library on `stream` wrote; records
+// `reads` ranges overlaps a range the previous launch of this library on `stream` of the current device
+// wrote (launch_record.h; false too where that launch is not on record and something is read); records
 // `writes` as what this launch writes (more than twelve ranges: the next launch is refused).
 // Invariant the staged kernels rely on: before its pdl_wait() a kernel reads weight bytes only, and
 // a weight range is only ever written by a copy (a stream-ordered memcpy is never overlapped) or by
