@@ -120,3 +120,35 @@ def test_values_at_the_ends_of_their_range(kind, exponent):
     y = Timed(t)
     y.call()
     assert near_rows(y.out.cpu().numpy(), t.want())
+
+
+@pytest.mark.parametrize("kind,n", [("f32", 1_300_003), ("fp8", 4_500_003)])
+@pytest.mark.parametrize("window", [0, 2000])
+def test_a_cache_beyond_32_bits_of_bytes(kind, n, window):
+    """Zero rows but for a few near and far, whose weights stand out: scores of 0 and values of 0 have a closed form."""
+    m, heads, kv_heads, d, cols = 3, 24, 4, 256, 1024
+    g = torch.Generator(device="cuda").manual_seed(7)
+    dtype = torch.float32 if kind == "f32" else torch.float8_e4m3fn
+    k, v = (torch.zeros(n + m, cols, dtype=dtype, device="cuda") for _ in range(2))
+    scale = None if kind == "f32" else torch.full((n + m,), 0.25, device="cuda")
+    assert k.numel() * k.element_size() > 2 ** 32
+    far = [5, n // 2, n - 1500, n - 1, *range(n, n + m)]
+    rows = [torch.randint(-7, 8, (2, cols), device="cuda", generator=g).float() for _ in far]
+    for j, (a, b) in zip(far, rows):
+        k[j], v[j] = a.to(dtype), b.to(dtype)
+    q = 2 * torch.randn(m, heads, d, device="cuda", generator=g) * (1.0 if kind == "f32" else 4.0)
+    parents, out = torch.arange(m, device="cuda", dtype=torch.int32) - 1, torch.zeros(m, heads, d, device="cuda")
+    s = None if scale is None else scale.data_ptr()
+    assert capi.load_library().tsr_attention_tree(FORMAT[kind], q.data_ptr(), k.data_ptr(), v.data_ptr(), s, s, parents.data_ptr(), out.data_ptr(), m, n, heads,
+                                                  kv_heads, d, 0, window, torch.cuda.current_stream().cuda_stream) == 0
+    unit, want = 1.0 if scale is None else 0.25, np.zeros((m, heads, d))
+    for i in range(m):
+        first = n + i + 1 - window if window else 0
+        seen = [x for j, x in zip(far, rows) if first <= j <= n + i]
+        keys, values = (unit * torch.stack([x[c] for x in seen]).double().view(-1, kv_heads, d).cpu().numpy() for c in (0, 1))
+        for h in range(heads):
+            scores = keys[:, h // 6] @ q[i, h].double().cpu().numpy() / np.sqrt(d)
+            top = max(0.0, scores.max())
+            w = np.exp(scores - top)
+            want[i, h] = w @ values[:, h // 6] / (w.sum() + (n + i + 1 - first - len(seen)) * np.exp(-top))
+    assert near_rows(out.cpu().numpy(), want, 1e-4)  # (scores of up to 40)
