@@ -24,7 +24,6 @@
 #include <cstdlib>
 #include <mutex>
 #include <unordered_map>
-#include <vector>
 #include <cuda_runtime.h>
 
 #include "codec.cuh"
